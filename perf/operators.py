@@ -266,10 +266,11 @@ def _plan_plain(s, lens, new, rows):
     n, most = table.shape
     i64 = torch.int64
     after = lens.to(i64) + new
-    want = torch.clamp((after + page - 1) // page - s["held"], min=0)
-    upto = torch.cumsum(want, 0)
     row_upto = torch.cumsum(new, 0)
-    fits = ((want == 0) | (upto <= s["free_count"])) & (after <= most * page) & (row_upto <= rows)
+    fits = (after <= most * page) & (row_upto <= rows)
+    want = torch.where(fits, torch.clamp((after + page - 1) // page - s["held"], min=0), 0)
+    upto = torch.cumsum(want, 0)
+    fits &= (want == 0) | (upto <= s["free_count"])
     want = torch.where(fits, want, 0)
     first = torch.cumsum(want, 0) - want
     col = torch.arange(most, device="cuda")[None, :]
