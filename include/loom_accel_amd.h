@@ -392,6 +392,128 @@ int loom_amd_model_position(const loom_amd_model* m);
  * sequence's last row after the final norm). */
 const float* loom_amd_model_last_hidden(const loom_amd_model* m);
 
+/* ---- serving many requests: paged 8-bit KV cache ---------------------- */
+/* No counterpart in the reference, whose cache is one fp32 ring per layer
+ * (poly/mha.go:95-96): these entry points let requests of different lengths
+ * share one cache and one call.  They allocate nothing and wait for nothing,
+ * so a stream that is being captured takes them.  Every pointer is memory of
+ * the current device; scratch and workspace belong to the call until it has
+ * run, so calls that may overlap (two streams, two captured graphs) need one
+ * each. */
+
+/* Tables of `requests` request slots over a pool of num_pages pages of
+ * page_size tokens (16, 32, 64 or 128).  Device buffers of the caller. */
+typedef struct loom_amd_page_table {
+    int32_t* pages;      /* requests x max_pages: page of positions [i*page_size, ..), -1: none */
+    int32_t* held;       /* requests: pages held */
+    int32_t* free_pages; /* num_pages: stack of the pages nobody holds */
+    int32_t* free_count; /* 1: its height */
+    int requests, max_pages, num_pages, page_size;
+} loom_amd_page_table;
+
+/* All pages free, no request holds any. */
+int loom_amd_page_table_reset(const loom_amd_page_table* table, void* stream);
+
+/* Device outputs of a plan. */
+typedef struct loom_amd_page_plan {
+    int32_t* row_start; /* requests + 1: first row of each request; the last: rows in use */
+    int32_t* lens;      /* requests: tokens with the new ones */
+    int32_t* request;   /* rows: request of each row, -1 behind the last */
+    int32_t* positions; /* rows: position in its request, -1: no place */
+    int32_t* slots;     /* rows: page * page_size + offset of that position, -1: no place */
+    int32_t* scratch;   /* 4 * requests, 16-byte aligned */
+} loom_amd_page_plan;
+
+/* Rows of a step that appends new_tokens[r] tokens to request r, which has
+ * lens[r] (both device, `requests` values; below 0 counts as 0): rows are
+ * numbered request by request, and pages that a request lacks are taken off the
+ * stack in request order.  Pages that it already holds serve again, so a plan
+ * from the same lens gives the same slots.  A request whose pages, table or
+ * rows do not suffice gets none: its lens stay and its rows are -1 (and the
+ * requests after it that need pages more than there are get none either).
+ * rows is the capacity of the row outputs. */
+int loom_amd_page_table_plan(const loom_amd_page_table* table, const int32_t* lens, const int32_t* new_tokens,
+                             int rows, const loom_amd_page_plan* plan, void* stream);
+
+/* Gives back the pages of every request r with done[r] != 0. */
+int loom_amd_page_table_release(const loom_amd_page_table* table, const uint8_t* done, void* stream);
+
+/* Keys and values as int8 codes with an fp32 scale for each page, head and
+ * side: value = code * scale.  Device buffers of the caller, codes 16-byte
+ * aligned; head_dim 32, 64, 128 or 256. */
+typedef struct loom_amd_kv_pages {
+    int8_t* k;      /* num_pages x kv_heads x page_size x head_dim */
+    int8_t* v;      /* num_pages x kv_heads x head_dim x page_size */
+    float* k_scale; /* num_pages x kv_heads */
+    float* v_scale; /* num_pages x kv_heads */
+    int num_pages, page_size, kv_heads, head_dim;
+} loom_amd_kv_pages;
+
+#define LOOM_AMD_ROW_F32 0
+#define LOOM_AMD_ROW_BF16 1
+#define LOOM_AMD_ROW_F64 2
+
+/* Quantizes rows of keys and values (rows x kv_heads x head_dim, row strides
+ * in elements) into their slots.  Scale of a page's head: the largest finite
+ * magnitude / 127 of what the page holds; a row at offset 0 starts its page
+ * anew.  code = round-half-away(x / scale), exactly; where a later row raises
+ * the scale, the codes before it are rounded again at the new one.  NaN is
+ * stored as 0, an infinity as the largest code; a block whose magnitudes are
+ * under 2^-100 is stored as zeros.  Rows with a slot outside the cache are
+ * skipped.  The rows of one page stand one after another with ascending slots
+ * (as a plan numbers them); no slot occurs twice in a call. */
+int loom_amd_kv_append(const loom_amd_kv_pages* cache, const void* k, const void* v, int type, int rows,
+                       int64_t k_stride, int64_t v_stride, const int32_t* slots, void* stream);
+
+/* The fp32 values of slots: k and v, rows x kv_heads x head_dim; zeros for a
+ * slot outside the cache. */
+int loom_amd_kv_read(const loom_amd_kv_pages* cache, const int32_t* slots, int rows, float* k, float* v,
+                     void* stream);
+
+/* Bytes of workspace of a loom_amd_paged_attention call (0: none needed). */
+int loom_amd_paged_attention_workspace(int rows, int heads, int kv_heads, int head_dim, int requests,
+                                       int max_context, size_t* bytes);
+
+/* Causal grouped-query attention of rows (fp32, bf16 or fp64; rows x heads x
+ * head_dim, row strides in elements) over the cache: row t of request r
+ * (row_start[r] <= t < row_start[r + 1]) attends to positions 0 ..
+ * positions[t] of r's pages (requests x max_pages).  One call takes single
+ * decode rows, chunks of prompts, or both.  Row and page numbers are checked
+ * on the device: a position past max_context - 1 counts as that one, tokens
+ * whose page is none of the cache's are left out, a row with nothing to attend
+ * to (position -1) gives zeros, rows of no request are left as they are, and a
+ * row with a query that is not finite gives NaN.  Scores, probabilities and
+ * sums are fp32 (fp64 rows are rounded to fp32 first). */
+int loom_amd_paged_attention(const loom_amd_kv_pages* cache, const int32_t* pages, int requests, int max_pages,
+                             const int32_t* row_start, const int32_t* positions, const void* q, int type, int rows,
+                             int heads, int64_t q_stride, float scale, int max_context, void* out,
+                             int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- sampling ---------------------------------------------------------- */
+
+#define LOOM_AMD_SAMPLE_MAX_VOCAB 8388608
+
+int loom_amd_sample_workspace(int vocab, int rows, size_t* bytes);
+
+/* One token per row of logits (fp32, `stride` elements apart) from uniform[r]
+ * in [0, 1): the sampling that SampleTopK (poly/sampling.go:44-55) does beyond
+ * its greedy pick, with the filters of current serving stacks.  temperature,
+ * top_k, top_p and min_p hold a value per row, or are NULL (1, off, off, off).
+ *   w_i = exp((l_i - max) / temperature), in fp64
+ *   tokens rank by logit, equal logits by index;
+ *   top_k > 0 keeps the first k; top_p < 1 keeps the shortest first part of
+ *   those whose mass is at least top_p of theirs; min_p > 0 keeps w_i >= min_p
+ *   (at most 1); the first token always stays;
+ *   ids[r] = the first token in vocabulary order at which the kept mass summed
+ *   from token 0 exceeds uniform[r] times the whole kept mass.
+ * temperature <= 0 (or NaN) picks as loom_amd_greedy_sample does.  A NaN logit
+ * is never drawn, +infinity counts as the largest finite value, and tokens more
+ * than 32 nats under the maximum have no mass.  The result does not depend on
+ * the order in which the device works. */
+int loom_amd_sample(const float* logits, int64_t stride, int vocab, int rows, const float* temperature,
+                    const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform,
+                    int32_t* ids, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

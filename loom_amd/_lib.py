@@ -17,6 +17,7 @@ _lib: C.CDLL | None = None
 
 P = C.c_void_p
 i32 = C.c_int
+i64 = C.c_int64
 f32 = C.c_float
 f64 = C.c_double
 sz = C.c_size_t
@@ -69,6 +70,24 @@ class ModelDesc(C.Structure):
     _fields_ = [("block", BlockDesc), ("num_layers", i32), ("vocab", i32),
                 ("final_norm_eps", f64), ("max_tokens", i32), ("max_prefill", i32),
                 ("lm_head_order", i32)]
+
+
+class PageTable(C.Structure):
+    """loom_amd_page_table."""
+    _fields_ = [("pages", P), ("held", P), ("free_pages", P), ("free_count", P),
+                ("requests", i32), ("max_pages", i32), ("num_pages", i32), ("page_size", i32)]
+
+
+class PagePlan(C.Structure):
+    """loom_amd_page_plan."""
+    _fields_ = [("row_start", P), ("lens", P), ("request", P), ("positions", P), ("slots", P),
+                ("scratch", P)]
+
+
+class KvPages(C.Structure):
+    """loom_amd_kv_pages."""
+    _fields_ = [("k", P), ("v", P), ("k_scale", P), ("v_scale", P),
+                ("num_pages", i32), ("page_size", i32), ("kv_heads", i32), ("head_dim", i32)]
 
 
 # name -> (restype, argtypes); every symbol declared in include/*.h.
@@ -127,6 +146,16 @@ SIGNATURES = {
     "loom_amd_model_tokens": (i32, [P, P, i32, P]),
     "loom_amd_model_position": (i32, [P]),
     "loom_amd_model_last_hidden": (P, [P]),
+    "loom_amd_page_table_reset": (i32, [C.POINTER(PageTable), P]),
+    "loom_amd_page_table_plan": (i32, [C.POINTER(PageTable), P, P, i32, C.POINTER(PagePlan), P]),
+    "loom_amd_page_table_release": (i32, [C.POINTER(PageTable), P, P]),
+    "loom_amd_kv_append": (i32, [C.POINTER(KvPages), P, P, i32, i32, i64, i64, P, P]),
+    "loom_amd_kv_read": (i32, [C.POINTER(KvPages), P, i32, P, P, P]),
+    "loom_amd_paged_attention_workspace": (i32, [i32, i32, i32, i32, i32, i32, C.POINTER(sz)]),
+    "loom_amd_paged_attention": (i32, [C.POINTER(KvPages), P, i32, i32, P, P, P, i32, i32, i32, i64, f32,
+                                       i32, P, i64, P, sz, P]),
+    "loom_amd_sample_workspace": (i32, [i32, i32, C.POINTER(sz)]),
+    "loom_amd_sample": (i32, [P, i64, i32, i32, P, P, P, P, P, P, P, sz, P]),
 }
 
 

@@ -1,0 +1,657 @@
+// paged_attention.hip -- causal attention of new rows over a paged cache of
+// int8 codes (paged.hpp): one kernel for single decode rows, chunks of a
+// prompt, and both in one call.
+//
+//   out[row, h] = sum_t p_t v_t / sum_t p_t,   p_t = exp(scale q.k_t - max)
+// over t <= position(row), with k_t = kc_t ks, v_t = vc_t vs of t's page.
+//
+// The matrix cores read the keys' codes as they are stored: q is written in
+// fixed point as QD signed 8-bit digits relative to its largest magnitude, and
+// v_mfma_i32_16x16x64_i8 forms every digit's dot product exactly in 32 bits;
+// the digits' sums are joined in fp32.  Three digits (23 bits and sign) leave
+// no more error than an fp32 q has; two (15 bits) stand far below a bf16 q's.
+// The values' codes become fp16 (exact) and meet p as one fp16 factor (bf16
+// rows) or as the sum of two (22 bits, fp32 rows).
+//
+// A wave owns 16 columns: (row, head of the group) pairs of one request and
+// key/value head.  It computes scores transposed, S^T = K Q^T, so lane (n, g)
+// (n = lane & 15, g = lane >> 4) holds column n's scores of the 16 tokens
+// 16g .. 16g+15 of a 64-token step: row r of the K operand of tile t is token
+// 16 (r >> 2) + 4 t + (r & 3).  That is the B operand of O^T = V^T P^T as it
+// stands, so probabilities never leave registers, nothing but the final join
+// uses LDS, and a lane's 16 tokens lie in one page: its scales are one factor.
+#include "paged.hpp"
+
+namespace lamd {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+constexpr int kStep = 64;         // tokens of one step
+constexpr int kMaxSplits = 64;    // parts of one context (a wave joins them, a lane each)
+constexpr float kPeak = 32768.0f; // fp16 value of a probability of 1
+constexpr float kNegInf = -__builtin_inff();
+
+struct AttnParams {
+    const int8_t* k;
+    const int8_t* v;
+    const float* ks;
+    const float* vs;
+    const int32_t* table;
+    const int32_t* row_start;
+    const int32_t* positions;
+    const void* q;
+    void* out;
+    float* part_o;    // [split][row][head][hd]
+    float* part_ml;   // [split][row][head][2]
+    int32_t* active;  // [row][head]: parts of this row's context
+    int pages, shift, kv_heads, max_pages, requests, rows, heads, group, splits, type, max_context;
+    int min_steps;       // steps of a part
+    int lo_cols, hi_cols;  // this launch takes requests with lo_cols <= columns <= hi_cols
+    long q_stride, out_stride;
+    float scale2;  // scale * log2(e)
+    bool vec;      // rows of q and out are 16-byte aligned
+};
+
+__device__ __forceinline__ float shfl_xor_f(float v, int m) { return __shfl_xor(v, m, 64); }
+
+__device__ __forceinline__ float bf16_f(uint32_t hi16) { return __uint_as_float(hi16 << 16); }
+
+__device__ __forceinline__ uint32_t f_bf16(float f) {  // round to nearest, ties to even; NaN stays NaN
+    const uint32_t u = __float_as_uint(f);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return (u >> 16) | 0x40u;
+    return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+}
+
+// 16 consecutive elements of a row as fp32.
+__device__ __forceinline__ void load16(const void* base, int type, long at, bool vec, float* x) {
+    if (type == ROW_BF16) {
+        const uint16_t* p = (const uint16_t*)base + at;
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint4 u = ((const uint4*)p)[i];
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    x[8 * i + 2 * j] = bf16_f(w[j] & 0xffffu);
+                    x[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = bf16_f(p[i]);
+        }
+    } else if (type == ROW_F32) {
+        const float* p = (const float*)base + at;
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 f = ((const float4*)p)[i];
+                x[4 * i] = f.x, x[4 * i + 1] = f.y, x[4 * i + 2] = f.z, x[4 * i + 3] = f.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = p[i];
+        }
+    } else {
+        const double* p = (const double*)base + at;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = (float)p[i];
+    }
+}
+
+// 4 consecutive elements of an output row.
+__device__ __forceinline__ void store4(void* base, int type, long at, bool vec, const float* x) {
+    if (type == ROW_BF16) {
+        uint16_t* p = (uint16_t*)base + at;
+        if (vec) {
+            *(uint2*)p = make_uint2(f_bf16(x[0]) | (f_bf16(x[1]) << 16), f_bf16(x[2]) | (f_bf16(x[3]) << 16));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = (uint16_t)f_bf16(x[i]);
+        }
+    } else if (type == ROW_F32) {
+        float* p = (float*)base + at;
+        if (vec) {
+            *(float4*)p = make_float4(x[0], x[1], x[2], x[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = x[i];
+        }
+    } else {
+        double* p = (double*)base + at;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = (double)x[i];
+    }
+}
+
+// Column tiles of `ct` columns: request r has the launch's tiles from
+// start_r * group / ct + r on (the sum of the earlier requests' rounded-up
+// tile counts is never more), so a tile finds its request by one search and no
+// list of tiles has to be built.  Returns the request or -1; a wave searches
+// 64 requests at a time.
+__device__ __forceinline__ int find_request(const AttnParams& a, int ct, int x, int lane, int* first_tile) {
+    int lo = 0, hi = a.requests;
+    while (true) {
+        const int step = (hi - lo + 63) >> 6;
+        const int r = lo + lane * step;
+        long f = 0;
+        if (r < hi) {
+            int s = a.row_start[r];
+            s = s < 0 ? 0 : (s > a.rows ? a.rows : s);
+            f = (long)s * a.group / ct + r;
+        }
+        const unsigned long long at_or_before = __ballot(r < hi && f <= x);
+        if (!at_or_before) return -1;
+        const int last = 63 - __builtin_clzll(at_or_before);
+        lo += last * step;
+        if (step == 1) {
+            *first_tile = __shfl((int)f, last, 64);
+            return lo;
+        }
+        hi = lo + step < hi ? lo + step : hi;
+    }
+}
+
+template <int HD, int QD, int PL>
+struct Wave {
+    static constexpr int NS = HD >= 64 ? HD / 64 : 1;  // 64-dimension steps of the score product
+    static constexpr int ND = HD / 16;                 // 16-dimension tiles of the output
+    v4i qd[QD][NS];
+    float qf;  // value of one unit of q's fixed point, with scale * log2(e)
+    v4f o[ND];
+    float m, l, ref;
+
+    // q's digits of this lane: column n's dimensions 64 s + 16 g ..
+    __device__ __forceinline__ void load_q(const AttnParams& a, long at, bool valid, int g) {
+        float x[NS][16];
+        float big = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            if (valid && 64 * s + 16 * g < HD) {
+                load16(a.q, a.type, at + 64 * s + 16 * g, a.vec, x[s]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[s][i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                bad = bad || !(fabsf(x[s][i]) <= 3.402823466e38f);
+                big = fmaxf(big, fabsf(x[s][i]));
+            }
+        }
+        big = fmaxf(big, shfl_xor_f(big, 16));
+        big = fmaxf(big, shfl_xor_f(big, 32));
+        float nan = bad ? __builtin_nanf("") : 0.0f;
+        nan += shfl_xor_f(nan, 16);
+        nan += shfl_xor_f(nan, 32);
+        // largest fixed-point value: just under the digits' own, 127 * (1 + 256 (+ 65536))
+        constexpr float kTop = QD == 3 ? 8355000.0f : 32600.0f;
+        const bool zero = big < 0x1p-100f;
+        const float inv = zero ? 0.0f : kTop / big;
+        qf = (zero ? 0.0f : big / kTop) * a.scale2 + nan;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t t[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float f = rintf(x[s][4 * w + i] * inv);
+                    f = fminf(fmaxf(f, -kTop), kTop);  // (NaN, infinities: any digits, qf is NaN)
+                    t[i] = ((uint32_t)(int)f + 0x80808080u) ^ 0x80808080u;  // signed digits, lowest byte first
+                }
+                const uint32_t a01 = __builtin_amdgcn_perm(t[1], t[0], 0x05010400u);
+                const uint32_t a23 = __builtin_amdgcn_perm(t[3], t[2], 0x05010400u);
+                qd[0][s][w] = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100u);
+                qd[1][s][w] = (int)__builtin_amdgcn_perm(a23, a01, 0x07060302u);
+                if (QD == 3) {
+                    const uint32_t b01 = __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0602u);
+                    const uint32_t b23 = __builtin_amdgcn_perm(t[3], t[2], 0x0c0c0602u);
+                    qd[QD - 1][s][w] = (int)__builtin_amdgcn_perm(b23, b01, 0x05040100u);
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        m = kNegInf;
+        l = 0.0f;
+        ref = 0x1p-100f;  // under every scale that holds a value
+    }
+
+    __device__ __forceinline__ static v4i ldg(const int8_t* p) { return *(const v4i*)p; }
+
+    // Codes of one step.
+    struct Codes {
+        v4i k[4][NS];
+        v4i v[ND];
+        float ks, vs;
+        bool ok;  // this lane's 16 tokens have a page
+    };
+
+    // Page of a token of request table `tab`, -1 when there is none.
+    __device__ __forceinline__ static int page_of(const AttnParams& a, const int32_t* tab, int tok, int npages) {
+        const int i = tok >> a.shift;
+        int id = -1;
+        if (i < npages) id = tab[i];
+        return (unsigned)id < (unsigned)a.pages ? id : -1;
+    }
+
+    __device__ __forceinline__ void load_codes(const AttnParams& a, const int32_t* tab, int tok0, int npages, int kvh,
+                                               int n, int g, Codes& c) {
+        const int tk = tok0 + 16 * (n >> 2), tv = tok0 + 16 * g;
+        const int idk = page_of(a, tab, tk, npages), idv = page_of(a, tab, tv, npages);
+        const int mask = (1 << a.shift) - 1;
+        // (no page: any page's codes are read in their place and masked)
+        const long bk = ((long)(idk < 0 ? 0 : idk) * a.kv_heads + kvh);
+        const long bv = ((long)(idv < 0 ? 0 : idv) * a.kv_heads + kvh);
+        c.ok = idv >= 0;
+        c.ks = a.ks[bv];
+        c.vs = idv < 0 ? 0.0f : a.vs[bv];
+        const int8_t* kp = a.k + ((bk << a.shift) + (tk & mask) + (n & 3)) * HD + 16 * g;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                if (HD >= 64 || 16 * g < HD) c.k[t][s] = ldg(kp + 4 * t * HD + 64 * s);
+                else c.k[t][s] = v4i{0, 0, 0, 0};
+            }
+        }
+        const int8_t* vp = a.v + ((bv * HD + n) << a.shift) + (tv & mask);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) c.v[d] = ldg(vp + ((long)(16 * d) << a.shift));
+    }
+
+    // Scores of a step, the running maximum and sum, and the value product.
+    __device__ __forceinline__ void step(const Codes& c, int tok0, int g, int limit, bool full) {
+        float x[16];
+        const float f = qf * c.ks;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            v4i acc[QD];
+#pragma unroll
+            for (int d = 0; d < QD; ++d) acc[d] = v4i{0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+#pragma unroll
+                for (int d = 0; d < QD; ++d)
+                    acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(c.k[t][s], qd[d][s], acc[d], 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float y = (float)acc[QD - 1][i];
+#pragma unroll
+                for (int d = QD - 2; d >= 0; --d) y = __builtin_fmaf(y, 256.0f, (float)acc[d][i]);
+                x[4 * t + i] = y * f;
+            }
+        }
+        if (!full) {
+            const int left = c.ok ? limit - (tok0 + 16 * g) : 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = i < left ? x[i] : kNegInf;
+        }
+        float mx = x[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+        mx = fmaxf(mx, shfl_xor_f(mx, 16));
+        mx = fmaxf(mx, shfl_xor_f(mx, 32));
+        float vmax = fmaxf(c.vs, shfl_xor_f(c.vs, 16));
+        vmax = fmaxf(vmax, shfl_xor_f(vmax, 32));
+        const float m_new = fmaxf(m, mx);
+        const float base = m_new == kNegInf ? 0.0f : m_new;
+        // the values' scales count relative to the largest so far, as a power of two
+        float ref_new = ref;
+        if (vmax > ref) ref_new = __uint_as_float(((__float_as_uint(vmax) >> 23) + 1) << 23);
+        if (__any(m_new > m || ref_new > ref)) {
+            const float al = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - base);
+            l *= al;
+            const float ao = al * (ref / ref_new);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] *= ao;
+            m = m_new;
+            ref = ref_new;
+        }
+        const float pf = c.vs * (kPeak / ref);
+        uint32_t hi[8], lo[8];
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float p0 = __builtin_amdgcn_exp2f(x[2 * i] - base), p1 = __builtin_amdgcn_exp2f(x[2 * i + 1] - base);
+            sum += p0 + p1;
+            const float w0 = p0 * pf, w1 = p1 * pf;
+            const v2h h = {(_Float16)w0, (_Float16)w1};
+            hi[i] = __builtin_bit_cast(uint32_t, h);
+            if (PL == 2) {
+                const v2h r = {(_Float16)(w0 - (float)h[0]), (_Float16)(w1 - (float)h[1])};
+                lo[i] = __builtin_bit_cast(uint32_t, r);
+            }
+        }
+        l += sum;
+        const v8h h0 = __builtin_bit_cast(v8h, v4i{(int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]});
+        const v8h h1 = __builtin_bit_cast(v8h, v4i{(int)hi[4], (int)hi[5], (int)hi[6], (int)hi[7]});
+        v8h l0, l1;
+        if (PL == 2) {
+            l0 = __builtin_bit_cast(v8h, v4i{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3]});
+            l1 = __builtin_bit_cast(v8h, v4i{(int)lo[4], (int)lo[5], (int)lo[6], (int)lo[7]});
+        }
+        const v2h bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            // code + 128 as the low bits of an fp16 of 1024, less 1152
+            v4i w[2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t u = (uint32_t)c.v[d][j] ^ 0x80808080u;
+                const v2h a = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias;
+                const v2h b = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias;
+                w[j >> 1][2 * (j & 1)] = (int)__builtin_bit_cast(uint32_t, a);
+                w[j >> 1][2 * (j & 1) + 1] = (int)__builtin_bit_cast(uint32_t, b);
+            }
+            const v8h v0 = __builtin_bit_cast(v8h, w[0]), v1 = __builtin_bit_cast(v8h, w[1]);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, h0, o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, h1, o[d], 0, 0, 0);
+            if (PL == 2) {
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, l0, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, l1, o[d], 0, 0, 0);
+            }
+        }
+    }
+};
+
+// out = o / l, zeros for a row that attends to nothing
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
+// WSPLIT: the workgroup's four waves share 16 columns and take every fourth
+// step (few columns: decode rows); otherwise each wave has its own 16 columns.
+// blockIdx.z is the part of the context.
+template <int HD, int QD, int PL, bool WSPLIT>
+__global__ __launch_bounds__(256) void paged_attn_kernel(AttnParams a) {
+    constexpr int CT = WSPLIT ? 16 : 64;
+    constexpr int LDO = HD + 4;
+    __shared__ __align__(16) float o_s[WSPLIT ? 4 * 16 * LDO : 1];
+    __shared__ float ml_s[WSPLIT ? 4 * 16 * 2 : 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.y, part = blockIdx.z;
+    int first_tile;
+    const int x = blockIdx.x;
+    const int r = find_request(a, CT, x, lane, &first_tile);
+    if (r < 0) return;
+    int start = a.row_start[r], end = a.row_start[r + 1];
+    start = start < 0 ? 0 : start;
+    end = end > a.rows ? a.rows : end;
+    const long cols = (long)(end - start) * a.group;
+    const long c0 = (long)(x - first_tile) * CT;
+    if (c0 >= cols || cols < a.lo_cols || cols > a.hi_cols) return;
+    const long col = c0 + (WSPLIT ? 0 : 16 * wave) + n;
+    const bool valid = col < cols;
+    const int row = start + (valid ? (int)(col / a.group) : 0);
+    const int head = kvh * a.group + (valid ? (int)(col % a.group) : 0);
+    int limit = 0;  // tokens this column attends to
+    if (valid) {
+        limit = a.positions[row] + 1;
+        limit = limit < 0 ? 0 : (limit > a.max_context ? a.max_context : limit);
+    }
+    int most = limit;
+    int least = valid ? limit : 0x7fffffff;
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) {
+        most = max(most, __shfl_xor(most, d, 64));
+        least = min(least, __shfl_xor(least, d, 64));
+    }
+    const int steps = (most + kStep - 1) / kStep;
+    int active = (steps + a.min_steps - 1) / a.min_steps;
+    active = active < 1 ? 1 : (active > a.splits ? a.splits : active);
+    const int per = (steps + active - 1) / active;
+    if (per > 0) active = (steps + per - 1) / per;
+    if (part >= active) return;
+    if (WSPLIT ? false : c0 + 16 * wave >= cols) return;
+
+    Wave<HD, QD, PL> w;
+    w.clear();
+    const long rh = (long)row * a.heads + head;
+    const int s0 = part * per, s1 = min(s0 + per, steps);
+    const int first = s0 + (WSPLIT ? wave : 0), stride = WSPLIT ? 4 : 1;
+    if (first < s1) {
+        const int32_t* tab = a.table + (long)r * a.max_pages;
+        const int npages = (most + (1 << a.shift) - 1) >> a.shift;
+        typename Wave<HD, QD, PL>::Codes c;
+        w.load_codes(a, tab, first * kStep, npages, kvh, n, g, c);
+        w.load_q(a, (long)row * a.q_stride + (long)head * HD, valid, g);
+        for (int s = first; s < s1; s += stride) {
+            const int tok0 = s * kStep;
+            const bool full = tok0 + kStep <= least && __all(c.ok);
+            w.step(c, tok0, g, limit, full);
+            if (s + stride < s1) w.load_codes(a, tab, (s + stride) * kStep, npages, kvh, n, g, c);
+        }
+    }
+    float l = w.l;
+    l += shfl_xor_f(l, 16);
+    l += shfl_xor_f(l, 32);
+    const float unit = w.ref * (1.0f / kPeak);
+    float* part_o = a.part_o + ((long)part * a.rows * a.heads + rh) * HD;
+    float* part_ml = a.part_ml + ((long)part * a.rows * a.heads + rh) * 2;
+    if (WSPLIT) {
+        // join the four waves' parts
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) {
+            const v4f y = w.o[d] * unit;
+            *(v4f*)&o_s[(wave * 16 + n) * LDO + 16 * d + 4 * g] = y;
+        }
+        if (g == 0) {
+            ml_s[(wave * 16 + n) * 2] = w.m;
+            ml_s[(wave * 16 + n) * 2 + 1] = l;
+        }
+        __syncthreads();
+        // thread t: column t / 16, dimensions 4 (t % 16) + 64 i
+        const int cn = threadIdx.x >> 4, d0 = 4 * (threadIdx.x & 15);
+        if (c0 + cn >= cols) return;
+        float m = kNegInf;
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, ml_s[(i * 16 + cn) * 2]);
+        float wt[4], sum = 0.0f;
+        for (int i = 0; i < 4; ++i) {
+            const float mi = ml_s[(i * 16 + cn) * 2];
+            wt[i] = mi == m ? 1.0f : __builtin_amdgcn_exp2f(mi - m);
+            sum += wt[i] * ml_s[(i * 16 + cn) * 2 + 1];
+        }
+        const int crow = start + (int)((c0 + cn) / a.group), chead = kvh * a.group + (int)((c0 + cn) % a.group);
+        const long crh = (long)crow * a.heads + chead;
+        const float inv = active == 1 ? inverse_sum(sum) : 1.0f;
+        for (int d = d0; d < HD; d += 64) {
+            float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < 4; ++i) {
+                const v4f p = *(const v4f*)&o_s[(i * 16 + cn) * LDO + d];
+                for (int j = 0; j < 4; ++j) y[j] += wt[i] * p[j];
+            }
+            for (int j = 0; j < 4; ++j) y[j] *= inv;
+            if (active == 1) store4(a.out, a.type, (long)crow * a.out_stride + (long)chead * HD + d, a.vec, y);
+            else *(float4*)&a.part_o[((long)part * a.rows * a.heads + crh) * HD + d] = make_float4(y[0], y[1], y[2], y[3]);
+        }
+        if ((threadIdx.x & 15) == 0 && a.splits > 1) {
+            if (active > 1) {
+                float* ml = a.part_ml + ((long)part * a.rows * a.heads + crh) * 2;
+                ml[0] = m;
+                ml[1] = sum;
+            }
+            if (part == 0) a.active[crh] = active;
+        }
+        return;
+    }
+    if (!valid) return;
+    if (active == 1) {
+        const float inv = inverse_sum(l) * unit;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) {
+            float y[4];
+            for (int j = 0; j < 4; ++j) y[j] = w.o[d][j] * inv;
+            store4(a.out, a.type, (long)row * a.out_stride + (long)head * HD + 16 * d + 4 * g, a.vec, y);
+        }
+    } else {
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) *(v4f*)&part_o[16 * d + 4 * g] = w.o[d] * unit;
+        if (g == 0) {
+            part_ml[0] = w.m;
+            part_ml[1] = l;
+        }
+    }
+    if (a.splits > 1 && part == 0 && g == 0) a.active[rh] = active;
+}
+
+// Joins the parts of rows whose context was cut: one wave per (row, head).
+template <int HD>
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnParams a) {
+    const int lane = threadIdx.x & 63;
+    const long rh = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long all = (long)a.rows * a.heads;
+    if (rh >= all) return;
+    const int row = (int)(rh / a.heads), head = (int)(rh % a.heads);
+    if (row >= a.row_start[a.requests] || row < a.row_start[0]) return;  // rows of no request: left as they are
+    const int active = a.active[rh];
+    if (active <= 1 || active > a.splits) return;
+    float m = kNegInf, l = 0.0f;
+    if (lane < active) {
+        m = a.part_ml[(lane * all + rh) * 2];
+        l = a.part_ml[(lane * all + rh) * 2 + 1];
+    }
+    float top = m;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, shfl_xor_f(top, d));
+    const float wt = lane < active ? (m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top)) : 0.0f;
+    float sum = wt * l;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) sum += shfl_xor_f(sum, d);
+    const float inv = inverse_sum(sum);
+    constexpr int LW = HD / 4 < 64 ? HD / 4 : 64;  // lanes of one part's row
+    constexpr int PAR = 64 / LW;                   // parts read at a time
+    const int d = 4 * (lane % LW);
+    v4f y = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < active; i += PAR) {
+        const int p = i + lane / LW;
+        const float wp = __shfl(wt, p < 64 ? p : 63, 64);
+        if (p < active) y += wp * *(const v4f*)&a.part_o[(p * all + rh) * HD + d];
+    }
+#pragma unroll
+    for (int s = 32; s >= LW; s >>= 1) {
+        for (int j = 0; j < 4; ++j) y[j] += shfl_xor_f(y[j], s);
+    }
+    if (lane < LW) {
+        float z[4];
+        for (int j = 0; j < 4; ++j) z[j] = y[j] * inv;
+        store4(a.out, a.type, (long)row * a.out_stride + (long)head * HD + d, a.vec, z);
+    }
+}
+
+// Parts of a context: enough workgroups to fill the chip several times over.
+constexpr int kWantGroups = 1024;
+constexpr int kMinSteps = 4;  // 256 tokens: a step for each wave of a decode workgroup
+
+static int splits_for(int rows, int heads, int kv_heads, int requests, int max_context) {
+    const long tiles = ceil_div(rows * (heads / kv_heads), 64);
+    const long groups = (tiles > requests ? tiles : (requests < rows ? requests : rows)) * kv_heads;
+    long s = (kWantGroups + groups - 1) / groups;
+    const long most = ceil_div(max_context, kMinSteps * kStep);
+    s = s > most ? most : s;
+    return (int)(s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : s));
+}
+
+struct PartLayout {
+    size_t o, ml, active, bytes;
+};
+
+static PartLayout part_layout(int rows, int heads, int hd, int splits) {
+    PartLayout p{0, 0, 0, 0};
+    if (splits <= 1) return p;
+    const size_t rh = (size_t)rows * heads;
+    auto pad = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    p.ml = pad(rh * splits * hd * 4);
+    p.active = p.ml + pad(rh * splits * 8);
+    p.bytes = p.active + pad(rh * 4);
+    return p;
+}
+
+size_t paged_attn_workspace(int rows, int heads, int kv_heads, int hd, int requests, int max_context) {
+    return part_layout(rows, heads, hd, splits_for(rows, heads, kv_heads, requests, max_context)).bytes;
+}
+
+template <int HD, int QD, int PL>
+static hipError_t launch_typed(AttnParams& a, hipStream_t s) {
+    const int group = a.group;
+    const long cols = (long)a.rows * group;
+    const int kAll = 0x7fffffff;
+    // requests of at most 16 columns (decode rows) take the wave-split kernel;
+    // where every request may be one, it takes all of them
+    const bool few = cols <= 16l * a.requests;
+    a.lo_cols = 1;
+    a.hi_cols = few ? kAll : 16;
+    hipLaunchKernelGGL((paged_attn_kernel<HD, QD, PL, true>),
+                       dim3((unsigned)(cols / 16 + a.requests), (unsigned)a.kv_heads, (unsigned)a.splits), dim3(256), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (!few) {
+        a.lo_cols = 17;
+        a.hi_cols = kAll;
+        hipLaunchKernelGGL((paged_attn_kernel<HD, QD, PL, false>),
+                           dim3((unsigned)(cols / 64 + a.requests), (unsigned)a.kv_heads, (unsigned)a.splits), dim3(256), 0, s, a);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (a.splits > 1) {
+        hipLaunchKernelGGL(paged_attn_join_kernel<HD>, dim3((unsigned)(((long)a.rows * a.heads + 3) / 4)), dim3(256), 0, s, a);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+hipError_t launch_paged_attn(const PagedAttn& p, hipStream_t s) {
+    AttnParams a{};
+    a.k = p.c.k;
+    a.v = p.c.v;
+    a.ks = p.c.k_scale;
+    a.vs = p.c.v_scale;
+    a.table = p.table;
+    a.row_start = p.row_start;
+    a.positions = p.positions;
+    a.q = p.q;
+    a.out = p.out;
+    a.pages = p.c.pages;
+    a.shift = __builtin_ctz((unsigned)p.c.page);
+    a.kv_heads = p.c.kv_heads;
+    a.max_pages = p.max_pages;
+    a.requests = p.requests;
+    a.rows = p.rows;
+    a.heads = p.heads;
+    a.group = p.heads / p.c.kv_heads;
+    a.type = p.type;
+    a.max_context = p.max_context;
+    a.min_steps = kMinSteps;
+    a.q_stride = p.q_stride;
+    a.out_stride = p.out_stride;
+    a.scale2 = p.scale * 1.44269504088896340736f;
+    const int size = p.type == ROW_BF16 ? 2 : (p.type == ROW_F32 ? 4 : 8);
+    a.vec = p.type != ROW_F64 && ((uintptr_t)p.q & 15) == 0 && ((uintptr_t)p.out & 15) == 0 &&
+            (p.q_stride * size) % 16 == 0 && (p.out_stride * size) % 16 == 0;
+    a.splits = splits_for(p.rows, p.heads, p.c.kv_heads, p.requests, p.max_context);
+    const PartLayout l = part_layout(p.rows, p.heads, p.c.hd, a.splits);
+    a.part_o = (float*)((char*)p.workspace + l.o);
+    a.part_ml = (float*)((char*)p.workspace + l.ml);
+    a.active = (int32_t*)((char*)p.workspace + l.active);
+#define ATTN(HD) \
+    case HD: return p.type == ROW_BF16 ? launch_typed<HD, 2, 1>(a, s) : launch_typed<HD, 3, 2>(a, s);
+    switch (p.c.hd) {
+        ATTN(32)
+        ATTN(64)
+        ATTN(128)
+        ATTN(256)
+        default: return hipErrorInvalidValue;
+    }
+#undef ATTN
+}
+
+}  // namespace lamd

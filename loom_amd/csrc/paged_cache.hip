@@ -1,0 +1,414 @@
+// paged_cache.hip -- the tables of a paged cache built on the device from
+// request lengths, rows of keys and values quantized into its pages, and read
+// back.
+#include "paged.hpp"
+
+namespace lamd {
+
+// ---- tables -----------------------------------------------------------------
+
+__global__ void page_reset_kernel(PageTables t) {
+    const long n = (long)t.requests * t.max_pages;
+    const long i0 = (long)blockIdx.x * blockDim.x + threadIdx.x, step = (long)gridDim.x * blockDim.x;
+    for (long i = i0; i < n; i += step) t.table[i] = -1;
+    for (long i = i0; i < t.requests; i += step) t.held[i] = 0;
+    for (long i = i0; i < t.pages; i += step) t.free_pages[i] = t.pages - 1 - (int)i;
+    if (i0 == 0) *t.free_count = t.pages;
+}
+
+hipError_t launch_page_reset(const PageTables& t, hipStream_t s) {
+    const long n = (long)t.requests * t.max_pages > t.pages ? (long)t.requests * t.max_pages : t.pages;
+    const long blocks = (n + 255) / 256;
+    hipLaunchKernelGGL(page_reset_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, s, t);
+    return hipGetLastError();
+}
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = kPlanThreads / 64;
+// One workgroup also fills the rows up to these counts (its row starts in LDS).
+constexpr int kFoldRequests = 4096;
+constexpr int kFoldRows = 4096;
+
+// Inclusive sum over the workgroup in thread order; every thread gets the total.
+__device__ __forceinline__ long long block_scan(long long v, long long* wave_sum, long long* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const long long o = __shfl_up(v, d, 64);
+        if (lane >= d) v += o;
+    }
+    __syncthreads();  // wave_sum of the previous call has been read
+    if (lane == 63) wave_sum[wave] = v;
+    __syncthreads();
+    long long before = 0, all = 0;
+    for (int w = 0; w < kPlanWaves; ++w) {
+        const long long x = wave_sum[w];
+        if (w < wave) before += x;
+        all += x;
+    }
+    *total = all;
+    return v + before;
+}
+
+// The rows of a step, request by request: row_start is the running sum of the
+// new tokens (held to `rows`), and a request takes ceil((len + new) / page) -
+// held pages off the top of the free stack, in request order, so the page ids
+// depend on nothing but the lengths.  A request takes part whole or not at
+// all: one whose pages, row or table space run out keeps its length, and its
+// rows get position and slot -1.  One workgroup, because the running sums are
+// serial: what it costs is the latency of its few dependent steps (64 requests
+// of a decode step).  FILL also writes the pages and rows; otherwise
+// page_fill_kernel does, one workgroup a request, from scratch {first
+// position or -1, pages taken, top of the stack at its first page, pages held
+// before}.
+template <bool FILL>
+__global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PageTables t, const int32_t* __restrict__ lens,
+                                                                 const int32_t* __restrict__ new_tokens, int rows,
+                                                                 PlanOut o) {
+    __shared__ long long sum_rows[kPlanWaves], sum_pages[kPlanWaves];
+    __shared__ int start_s[FILL ? kFoldRequests + 1 : 1];
+    __shared__ int base_s[FILL ? kFoldRequests : 1];
+    __shared__ int taken_s;
+    const int tid = threadIdx.x;
+    const long long free0 = *t.free_count;
+    const long long room = (long long)t.max_pages * t.page;
+    long long rows_before = 0, pages_before = 0;
+    if (tid == 0) {
+        taken_s = 0;
+        o.row_start[0] = 0;
+        if (FILL) start_s[0] = 0;
+    }
+    for (int r0 = 0; r0 < t.requests; r0 += kPlanThreads) {
+        const int r = r0 + tid;
+        const bool in = r < t.requests;
+        long long base = 0, n = 0;
+        int held = 0;
+        if (in) {
+            base = lens[r] > 0 ? lens[r] : 0;
+            n = new_tokens[r] > 0 ? new_tokens[r] : 0;
+            held = t.held[r];
+        }
+        long long total;
+        const long long row_end = block_scan(n, sum_rows, &total) + rows_before;
+        rows_before += total;
+        bool ok = base + n <= room && row_end <= rows;
+        long long want = 0;
+        if (ok && in) {
+            want = (base + n + t.page - 1) / t.page - held;
+            if (want < 0) want = 0;
+        }
+        const long long page_end = block_scan(want, sum_pages, &total) + pages_before;
+        pages_before += total;
+        ok = ok && (want == 0 || page_end <= free0);
+        if (!ok) want = 0;
+        if (in) {
+            const int end = (int)(row_end < rows ? row_end : rows);
+            const int top = (int)(free0 - 1 - (page_end - want));
+            o.row_start[r + 1] = end;
+            o.lens[r] = (int32_t)(ok ? base + n : base);
+            if (FILL) {
+                start_s[r + 1] = end;
+                base_s[r] = ok ? (int)base : -1;
+                t.held[r] = held + (int)want;
+            } else {
+                int4 sc = make_int4(ok ? (int)base : -1, (int)want, top, held);
+                ((int4*)o.scratch)[r] = sc;
+            }
+            if (want > 0) atomicMax(&taken_s, (int)page_end);
+            if (FILL && want <= 16) {
+                for (int j = 0; j < (int)want; ++j) t.table[(long)r * t.max_pages + held + j] = t.free_pages[top - j];
+            }
+        }
+        if (FILL) {  // requests of many pages: a wave each
+            unsigned long long many = __ballot(in && want > 16);
+            while (many) {
+                const int l = __builtin_ctzll(many);
+                many &= many - 1;
+                const int w = __shfl((int)want, l, 64), h = __shfl(held, l, 64);
+                const int top = __shfl((int)(free0 - 1 - (page_end - want)), l, 64);
+                const long at = (long)(r0 + (tid & ~63) + l) * t.max_pages + h;
+                for (int j = tid & 63; j < w; j += 64) t.table[at + j] = t.free_pages[top - j];
+            }
+        }
+    }
+    __syncthreads();
+    if (tid == 0) *t.free_count = (int32_t)(free0 - taken_s);
+    if (FILL) {
+        for (int row = tid; row < rows; row += kPlanThreads) {
+            // the request whose rows hold this one: the last start at or before it
+            int lo = 0, hi = t.requests + 1;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (start_s[mid] <= row) lo = mid;
+                else hi = mid;
+            }
+            int req = -1, pos = -1, slot = -1;
+            if (lo < t.requests) {
+                req = lo;
+                if (base_s[lo] >= 0) {
+                    pos = base_s[lo] + row - start_s[lo];
+                    slot = t.table[(long)lo * t.max_pages + pos / t.page] * t.page + pos % t.page;
+                }
+            }
+            o.request[row] = req;
+            o.positions[row] = pos;
+            o.slots[row] = slot;
+        }
+    }
+}
+
+// Pages and rows of request blockIdx.x (the last block: rows behind the last
+// request), from page_plan_kernel's scratch.
+__global__ __launch_bounds__(256) void page_fill_kernel(PageTables t, int rows, PlanOut o) {
+    const int r = blockIdx.x;
+    const int first = threadIdx.x + blockIdx.y * blockDim.x, step = blockDim.x * gridDim.y;
+    if (r == t.requests) {
+        for (long row = (long)o.row_start[r] + first; row < rows; row += step) {
+            o.request[row] = o.positions[row] = o.slots[row] = -1;
+        }
+        return;
+    }
+    const int4 sc = ((const int4*)o.scratch)[r];
+    const int base = sc.x, want = sc.y, top = sc.z, held = sc.w;
+    int32_t* table = t.table + (long)r * t.max_pages;
+    for (int j = first; j < want; j += step) table[held + j] = t.free_pages[top - j];
+    if (want > 0 && first == 0) t.held[r] = held + want;
+    const int start = o.row_start[r], end = o.row_start[r + 1];
+    for (int row = start + first; row < end; row += step) {
+        int pos = -1, slot = -1;
+        if (base >= 0) {
+            pos = base + row - start;
+            const int i = pos / t.page;
+            slot = (i < held ? table[i] : t.free_pages[top - (i - held)]) * t.page + pos % t.page;
+        }
+        o.request[row] = r;
+        o.positions[row] = pos;
+        o.slots[row] = slot;
+    }
+}
+
+hipError_t launch_page_plan(const PageTables& t, const int32_t* lens, const int32_t* new_tokens, int rows,
+                            const PlanOut& o, hipStream_t s) {
+    if (t.requests <= kFoldRequests && rows <= kFoldRows) {
+        hipLaunchKernelGGL(page_plan_kernel<true>, dim3(1), dim3(kPlanThreads), 0, s, t, lens, new_tokens, rows, o);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL(page_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, s, t, lens, new_tokens, rows, o);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    // long requests spread over several workgroups
+    int parts = rows / (1024 * (t.requests < 64 ? t.requests : 64));
+    parts = parts < 1 ? 1 : (parts > 64 ? 64 : parts);
+    hipLaunchKernelGGL(page_fill_kernel, dim3((unsigned)t.requests + 1, parts), dim3(256), 0, s, t, rows, o);
+    return hipGetLastError();
+}
+
+// Pages of the requests marked done go back on the stack, in request order.
+__global__ __launch_bounds__(kPlanThreads) void page_release_kernel(PageTables t, const uint8_t* __restrict__ done) {
+    __shared__ long long sum[kPlanWaves];
+    const int tid = threadIdx.x;
+    const int free0 = *t.free_count;
+    long long before = 0;
+    for (int r0 = 0; r0 < t.requests; r0 += kPlanThreads) {
+        const int r = r0 + tid;
+        int n = 0;
+        if (r < t.requests && done[r]) {
+            n = t.held[r];
+            if (n > t.max_pages) n = t.max_pages;
+        }
+        long long total;
+        const long long at = block_scan(n, sum, &total) + before - n;
+        before += total;
+        if (n > 0) t.held[r] = 0;
+        unsigned long long some = __ballot(n > 0);
+        while (some) {
+            const int l = __builtin_ctzll(some);
+            some &= some - 1;
+            const int cnt = __shfl(n, l, 64);
+            const long long to = free0 + __shfl(at, l, 64);
+            int32_t* row = t.table + (long)(r0 + (tid & ~63) + l) * t.max_pages;
+            for (int j = tid & 63; j < cnt; j += 64) {
+                if (to + j < t.pages) t.free_pages[to + j] = row[j];
+                row[j] = -1;
+            }
+        }
+    }
+    __syncthreads();
+    if (tid == 0) *t.free_count = (int32_t)(free0 + before < t.pages ? free0 + before : t.pages);
+}
+
+hipError_t launch_page_release(const PageTables& t, const uint8_t* done, hipStream_t s) {
+    hipLaunchKernelGGL(page_release_kernel, dim3(1), dim3(kPlanThreads), 0, s, t, done);
+    return hipGetLastError();
+}
+
+// ---- append and read ------------------------------------------------------------
+
+constexpr float kMaxFinite = 3.402823466e38f;
+constexpr float kTinyAmax = 0x1p-100f;  // below it a block's values are zeros: its scale keeps full precision
+
+template <typename T>
+__device__ __forceinline__ float as_f32(T v);
+template <>
+__device__ __forceinline__ float as_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float as_f32<uint16_t>(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+
+__device__ __forceinline__ float finite_abs(float x) {
+    const float a = fabsf(x);
+    return a <= kMaxFinite ? a : 0.0f;  // NaN and infinities have no part in the scale
+}
+
+// round-half-away(x / s) exactly: the estimate is at most one off, and the
+// sign of |x| - (c +- 1/2) s, one fused operation, is exact (s >= 2^-107).
+// NaN gives 0, an infinity the largest code.
+__device__ __forceinline__ int code_of(float x, float s, float inv) {
+    const float a = fabsf(x);
+    if (!(a <= kMaxFinite)) return (a != a || s == 0.0f) ? 0 : (x > 0 ? 127 : -127);
+    float c = floorf(a * inv + 0.5f);
+    if (__builtin_fmaf(-(c - 0.5f), s, a) < 0.0f) c -= 1.0f;
+    else if (__builtin_fmaf(-(c + 0.5f), s, a) >= 0.0f) c += 1.0f;
+    const int i = (int)fminf(c, 127.0f);
+    return x < 0 ? -i : i;
+}
+
+// A code of scale `from` at the larger scale `to` (fp64: the product is exact).
+__device__ __forceinline__ int recode(int c, float from, float to) {
+    const double q = (double)c * (double)from / (double)to;
+    const int i = (int)floor(fabs(q) + 0.5);
+    return q < 0 ? -i : i;
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
+    return v;
+}
+
+// One wave per (run, head, side).  A run is the consecutive rows whose slots
+// follow one another within one page; the wave of a run's first row does all
+// of it, the others leave at once.  The page's scale is the larger of what it
+// had (unless the run starts the page: then nothing of it counts any more)
+// and the run's largest magnitude / 127.  When it grows, the codes of the
+// earlier tokens are rounded again at the new scale.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void kv_append_kernel(KvPages c, const T* __restrict__ k, const T* __restrict__ v,
+                                                        int rows, long k_stride, long v_stride,
+                                                        const int32_t* __restrict__ slots) {
+    const int lane = threadIdx.x & 63;
+    const int row = blockIdx.x;
+    const int job = blockIdx.y * 4 + (threadIdx.x >> 6);
+    if (job >= 2 * c.kv_heads) return;
+    const int head = job >> 1;
+    const bool is_v = job & 1;
+    const int slot = slots[row];
+    if (slot < 0 || slot >= c.pages * c.page) return;
+    const int page = slot / c.page, off = slot % c.page;
+    if (row > 0 && off > 0 && slots[row - 1] == slot - 1) return;  // not a run's first row
+    int n = 0;  // tokens of the run
+    for (int base = 0; base < c.page; base += 64) {
+        const int t = base + lane;
+        const bool more = row + t < rows && off + t < c.page && slots[row + t] == slot + t;
+        const unsigned long long m = ~__ballot(more);
+        if (m) {
+            n = base + __builtin_ctzll(m);
+            break;
+        }
+        n = base + 64;
+    }
+    const T* src = (is_v ? v + (long)row * v_stride : k + (long)row * k_stride) + head * HD;
+    const long stride = is_v ? v_stride : k_stride;
+    float* scale_at = (is_v ? c.v_scale : c.k_scale) + (long)page * c.kv_heads + head;
+    float big = 0.0f;
+    // HD is a power of two: a wave reads 64 consecutive values of a row, or
+    // several rows where one has fewer
+    for (int i = lane; i < n * HD; i += 64) big = fmaxf(big, finite_abs(as_f32<T>(src[(long)(i / HD) * stride + i % HD])));
+    big = wave_max(big);
+    const float from = off == 0 ? 0.0f : *scale_at;
+    const float own = big < kTinyAmax ? 0.0f : big / 127.0f;
+    const float to = fmaxf(from, own);
+    const float inv = to > 0.0f ? 1.0f / to : 0.0f;
+    const bool grows = off > 0 && to > from;
+    int8_t* codes = (is_v ? c.v : c.k) + ((long)page * c.kv_heads + head) * (long)(c.page * HD);
+    if (!is_v) {
+        if (grows) {
+            for (int i = lane; i < off * HD; i += 64) codes[i] = (int8_t)recode(codes[i], from, to);
+        }
+        for (int i = lane; i < n * HD; i += 64) {
+            const float x = as_f32<T>(src[(long)(i / HD) * stride + i % HD]);
+            codes[off * HD + i] = (int8_t)(to > 0.0f ? code_of(x, to, inv) : 0);
+        }
+    } else {
+        // four tokens of one dimension are one word
+        const int q0 = grows ? 0 : off >> 2, q1 = (off + n + 3) >> 2;
+        for (int i = lane; i < (q1 - q0) * HD; i += 64) {
+            const int d = i % HD, q = q0 + i / HD;
+            uint32_t* at = (uint32_t*)(codes + (long)d * c.page + 4 * q);
+            const bool whole = 4 * q >= off && 4 * q + 4 <= off + n;
+            uint32_t w = whole ? 0u : *at;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int t = 4 * q + b - off;
+                int code = (int8_t)(w >> (8 * b));
+                if (t < 0) {
+                    if (grows) code = recode(code, from, to);
+                } else if (t < n) {
+                    code = to > 0.0f ? code_of(as_f32<T>(src[(long)t * stride + d]), to, inv) : 0;
+                }
+                w = (w & ~(0xffu << (8 * b))) | ((uint32_t)(uint8_t)code << (8 * b));
+            }
+            *at = w;
+        }
+    }
+    if (lane == 0) *scale_at = to;
+}
+
+template <typename T>
+static hipError_t append_typed(const KvPages& c, const void* k, const void* v, int rows, long ks, long vs,
+                               const int32_t* slots, hipStream_t s) {
+    const dim3 grid((unsigned)rows, (unsigned)ceil_div(2 * c.kv_heads, 4));
+#define APPEND(HD)                                                                                                \
+    case HD:                                                                                                      \
+        hipLaunchKernelGGL((kv_append_kernel<T, HD>), grid, dim3(256), 0, s, c, (const T*)k, (const T*)v, rows, ks, \
+                           vs, slots);                                                                            \
+        break;
+    switch (c.hd) {
+        APPEND(32)
+        APPEND(64)
+        APPEND(128)
+        APPEND(256)
+        default: return hipErrorInvalidValue;
+    }
+#undef APPEND
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_append(const KvPages& c, const void* k, const void* v, int type, int rows, long k_stride,
+                            long v_stride, const int32_t* slots, hipStream_t s) {
+    return type == ROW_BF16 ? append_typed<uint16_t>(c, k, v, rows, k_stride, v_stride, slots, s)
+                            : append_typed<float>(c, k, v, rows, k_stride, v_stride, slots, s);
+}
+
+// Values code * scale of given slots; no slot reads as zeros.
+__global__ __launch_bounds__(256) void kv_read_kernel(KvPages c, const int32_t* __restrict__ slots,
+                                                      float* __restrict__ k, float* __restrict__ v) {
+    const int row = blockIdx.x;
+    const int slot = slots[row];
+    const bool in = slot >= 0 && slot < c.pages * c.page;
+    const int page = in ? slot / c.page : 0, off = in ? slot % c.page : 0;
+    for (int i = threadIdx.x; i < c.kv_heads * c.hd; i += blockDim.x) {
+        const int h = i / c.hd, d = i % c.hd;
+        const long ph = (long)page * c.kv_heads + h;
+        const long block = ph * ((long)c.page * c.hd);
+        const long at = (long)row * c.kv_heads * c.hd + i;
+        k[at] = in ? (float)c.k[block + (long)off * c.hd + d] * c.k_scale[ph] : 0.0f;
+        v[at] = in ? (float)c.v[block + (long)d * c.page + off] * c.v_scale[ph] : 0.0f;
+    }
+}
+
+hipError_t launch_kv_read(const KvPages& c, const int32_t* slots, int rows, float* k, float* v, hipStream_t s) {
+    hipLaunchKernelGGL(kv_read_kernel, dim3((unsigned)rows), dim3(256), 0, s, c, slots, k, v);
+    return hipGetLastError();
+}
+
+}  // namespace lamd

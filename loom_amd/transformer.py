@@ -22,6 +22,7 @@ the stream only).  There is no CPU fallback: a missing library raises.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass
 
 import numpy as np
@@ -270,6 +271,55 @@ def greedy_sample(logits):
     return ids
 
 
+@functools.lru_cache(maxsize=4096)
+def _sample_workspace(vocab: int, rows: int) -> int:
+    n = C.c_size_t()
+    check(_lib.lib().loom_amd_sample_workspace(vocab, rows, C.byref(n)), "sample")
+    return n.value
+
+
+def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None):
+    """One token per row of logits (float32 device tensor [rows, vocab], rows
+    dense, any row stride) from uniform [rows] in [0, 1) -> int32 ids.
+
+    temperature, top_p, min_p (float32) and top_k (int32) are device tensors of
+    one value per row, or None (1, off, off, off).  A temperature <= 0 picks
+    greedily.  The filters keep first parts of the tokens ranked by logit (equal
+    ones by index): top_k > 0 the first k; top_p < 1 the shortest part of those
+    whose mass is at least top_p of theirs; min_p > 0 those whose probability is
+    at least min_p times the largest.  The id is the first token in vocabulary
+    order at which the kept mass passes uniform times the whole
+    (loom_amd_sample)."""
+    torch = _torch()
+    if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_cuda:
+        raise ValueError("logits must be a float32 device tensor [rows, vocab]")
+    rows, vocab = logits.shape
+    if vocab == 0 or (logits.stride(1) != 1 and vocab > 1) or (rows > 1 and logits.stride(0) < vocab):
+        raise ValueError("logits: each row must be dense, and rows must not overlap")
+    dev = logits.device.index
+    args = []
+    for name, t, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                        ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32),
+                        ("uniform", uniform, torch.float32)):
+        if t is None and name != "uniform":
+            args.append(None)
+            continue
+        if t.dtype != dt or t.device != logits.device or t.shape != (rows,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {str(dt).split('.')[-1]} tensor of {rows} values on "
+                             f"the logits' device")
+        args.append(t.data_ptr())
+    ids = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    need = _sample_workspace(vocab, rows)
+    ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    call = (logits.data_ptr(), logits.stride(0), vocab, rows, *args, ids.data_ptr(), ws.data_ptr(), need)
+    if torch.cuda.current_device() == dev:
+        check(_lib.lib().loom_amd_sample(*call, _stream(dev)), "sample")
+    else:
+        with torch.cuda.device(dev):
+            check(_lib.lib().loom_amd_sample(*call, _stream(dev)), "sample")
+    return ids
+
+
 class Transformer:
     """A stack of BitNet blocks with fp32 embeddings, final RMSNorm and LM head
     (tied to the embeddings when lm_head is None), decoding greedily.  An fp32
@@ -364,4 +414,4 @@ class Transformer:
 
 
 __all__ = ["BlockConfig", "BlockWeights", "BlockTaps", "BitNetBlock", "Transformer", "NORM_STRICT",
-           "lm_head", "lm_head_sequential", "greedy_sample"]
+           "lm_head", "lm_head_sequential", "greedy_sample", "sample"]
