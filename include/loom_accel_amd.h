@@ -442,8 +442,8 @@ int loom_amd_page_table_release(const loom_amd_page_table* table, const uint8_t*
  * side: value = code * scale.  Device buffers of the caller, codes 16-byte
  * aligned; head_dim 32, 64, 128 or 256. */
 typedef struct loom_amd_kv_pages {
-    int8_t* k;      /* num_pages x kv_heads x page_size x head_dim */
-    int8_t* v;      /* num_pages x kv_heads x head_dim x page_size */
+    int8_t* k;      /* num_pages x kv_heads x page_size/16 x head_dim/16 x 16 tokens x 16 */
+    int8_t* v;      /* num_pages x kv_heads x page_size/16 x head_dim x 16 tokens */
     float* k_scale; /* num_pages x kv_heads */
     float* v_scale; /* num_pages x kv_heads */
     int num_pages, page_size, kv_heads, head_dim;
@@ -461,12 +461,12 @@ typedef struct loom_amd_kv_pages {
  * stored as 0, an infinity as the largest code; a block whose magnitudes are
  * under 2^-100 is stored as zeros.  Rows with a slot outside the cache are
  * skipped.  The rows of one page stand one after another with ascending slots
- * (as a plan numbers them); no slot occurs twice in a call. */
+ * (as a plan numbers them, without a gap); no slot occurs twice in a call. */
 int loom_amd_kv_append(const loom_amd_kv_pages* cache, const void* k, const void* v, int type, int rows,
                        int64_t k_stride, int64_t v_stride, const int32_t* slots, void* stream);
 
-/* The fp32 values of slots: k and v, rows x kv_heads x head_dim; zeros for a
- * slot outside the cache. */
+/* The fp32 values of slots: k and v, rows x kv_heads x head_dim, 16-byte
+ * aligned; zeros for a slot outside the cache. */
 int loom_amd_kv_read(const loom_amd_kv_pages* cache, const int32_t* slots, int rows, float* k, float* v,
                      void* stream);
 

@@ -3,9 +3,13 @@
 //
 // The cache holds int8 codes in pages of `page` tokens (16, 32, 64 or 128) with
 // one fp32 scale per page, key/value head and side; a value is code * scale.
-//   k codes: [pages][kv_heads][page][head_dim]
-//   v codes: [pages][kv_heads][head_dim][page]  (tokens contiguous: the value
-//            product of attention reads 16 tokens of one dimension at a time)
+//   k codes: [pages][kv_heads][page / 16][head_dim / 16][16 tokens][16 dimensions]
+//   v codes: [pages][kv_heads][page / 16][head_dim][16 tokens]
+// (blocks of 16 tokens in the order in which the matrix operands of attention
+// take them: the 16 bytes of neighbouring lanes lie side by side.  Keys token by
+// token put each lane's 16 bytes into a line of its own, 64 cache accesses a
+// load instead of 16, and bound the kernel by the L1: four prompts of 2048
+// tokens 310 us)
 //   scales:  [pages][kv_heads]
 // A slot is page * page_size + offset; -1 (and anything outside the cache) is
 // no slot.
@@ -22,6 +26,14 @@ struct KvPages {
     float* v_scale;
     int pages, page, kv_heads, hd;
 };
+
+// Offsets within a page's head (page * hd codes).
+__host__ __device__ inline int k_offset(int token, int d, int hd) {
+    return (token >> 4) * 16 * hd + (d >> 4) * 256 + (token & 15) * 16 + (d & 15);
+}
+__host__ __device__ inline int v_offset(int token, int d, int hd) {
+    return (token >> 4) * 16 * hd + d * 16 + (token & 15);
+}
 
 enum RowType : int { ROW_F32 = 0, ROW_BF16 = 1, ROW_F64 = 2 };
 

@@ -93,6 +93,7 @@ int loom_amd_kv_read(const loom_amd_kv_pages* cache, const int32_t* slots, int r
     if (rows < 0) return fail("bad shape");
     if (rows == 0) return 0;
     if (!slots || !k || !v) return fail("null buffer");
+    if (((uintptr_t)k & 15) || ((uintptr_t)v & 15)) return fail("outputs of kv_read must be 16-byte aligned");
     hipError_t e = launch_kv_read(c, slots, rows, k, v, (hipStream_t)stream);
     return e == hipSuccess ? 0 : fail_hip("kv_read", e);
 }

@@ -31,7 +31,12 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kStep = 64;         // tokens of one step
 constexpr int kMaxSplits = 64;    // parts of one context (a wave joins them, a lane each)
-constexpr float kPeak = 32768.0f; // fp16 value of a probability of 1
+// fp16 value of a probability of 1, and how far (log2) a score may pass the
+// maximum that the sums are relative to before they are rescaled: 2^(9 + 6)
+// stays in fp16's range, and few steps rescale
+constexpr float kPeak = 512.0f;
+constexpr float kSlack = 6.0f;
+constexpr float kHuge = 0x1p22f;  // scores from which the fused difference to the maximum is too coarse
 constexpr float kNegInf = -__builtin_inff();
 
 struct AttnParams {
@@ -54,6 +59,15 @@ struct AttnParams {
     float scale2;  // scale * log2(e)
     bool vec;      // rows of q and out are 16-byte aligned
 };
+
+// Largest over the four lanes that share a column (lanes n + 16 g): the
+// exchange instructions swap rows of 16 and halves in registers.
+__device__ __forceinline__ float column_max(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 
 __device__ __forceinline__ float shfl_xor_f(float v, int m) { return __shfl_xor(v, m, 64); }
 
@@ -163,7 +177,9 @@ struct Wave {
     v4i qd[QD][NS];
     float qf;  // value of one unit of q's fixed point, with scale * log2(e)
     v4f o[ND];
-    float m, l, ref;
+    // maximum that the sums are relative to (base: 0 for none yet), sum, largest
+    // scale of values, fp16 value of a probability of 1 at a scale of 1
+    float m, base, l, ref, unit;
 
     // q's digits of this lane: column n's dimensions 64 s + 16 g ..
     __device__ __forceinline__ void load_q(const AttnParams& a, long at, bool valid, int g) {
@@ -192,8 +208,9 @@ struct Wave {
         // largest fixed-point value: just under the digits' own, 127 * (1 + 256 (+ 65536))
         constexpr float kTop = QD == 3 ? 8355000.0f : 32600.0f;
         const bool zero = big < 0x1p-100f;
-        const float inv = zero ? 0.0f : kTop / big;
-        qf = (zero ? 0.0f : big / kTop) * a.scale2 + nan;
+        const float inv = zero ? 0.0f : (a.scale2 < 0.0f ? -kTop : kTop) / big;
+        qf = (zero ? 0.0f : big / kTop) * fabsf(a.scale2);
+        l += nan;  // a query that is not finite: NaN to the end
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
 #pragma unroll
@@ -222,57 +239,77 @@ struct Wave {
 #pragma unroll
         for (int i = 0; i < ND; ++i) o[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         m = kNegInf;
+        base = 0.0f;
         l = 0.0f;
         ref = 0x1p-100f;  // under every scale that holds a value
+        unit = kPeak / ref;
     }
 
     __device__ __forceinline__ static v4i ldg(const int8_t* p) { return *(const v4i*)p; }
 
-    // Codes of one step.
+    // Codes of one step, the scales of this lane's page, and whether it has one.
     struct Codes {
         v4i k[4][NS];
         v4i v[ND];
         float ks, vs;
-        bool ok;  // this lane's 16 tokens have a page
+        bool ok;
+    };
+    // Pages of this lane's key row and of its 16 tokens (-1: none).
+    struct Pages {
+        int k, v;
     };
 
-    // Page of a token of request table `tab`, -1 when there is none.
+    // (always a load, of the last page's number where tok is past it: a branch
+    // here would make the loop wait for every load it has under way)
     __device__ __forceinline__ static int page_of(const AttnParams& a, const int32_t* tab, int tok, int npages) {
-        const int i = tok >> a.shift;
-        int id = -1;
-        if (i < npages) id = tab[i];
-        return (unsigned)id < (unsigned)a.pages ? id : -1;
+        const unsigned i = (unsigned)tok >> a.shift;
+        const int id = tab[min(i, (unsigned)npages - 1)];
+        return i < (unsigned)npages ? id : -1;
     }
 
-    __device__ __forceinline__ void load_codes(const AttnParams& a, const int32_t* tab, int tok0, int npages, int kvh,
-                                               int n, int g, Codes& c) {
-        const int tk = tok0 + 16 * (n >> 2), tv = tok0 + 16 * g;
-        const int idk = page_of(a, tab, tk, npages), idv = page_of(a, tab, tv, npages);
-        const int mask = (1 << a.shift) - 1;
-        // (no page: any page's codes are read in their place and masked)
-        const long bk = ((long)(idk < 0 ? 0 : idk) * a.kv_heads + kvh);
-        const long bv = ((long)(idv < 0 ? 0 : idv) * a.kv_heads + kvh);
-        c.ok = idv >= 0;
-        c.ks = a.ks[bv];
-        c.vs = idv < 0 ? 0.0f : a.vs[bv];
-        const int8_t* kp = a.k + ((bk << a.shift) + (tk & mask) + (n & 3)) * HD + 16 * g;
+    __device__ __forceinline__ static Pages pages_of(const AttnParams& a, const int32_t* tab, int tok0, int npages, int n,
+                                                     int g) {
+        return Pages{page_of(a, tab, tok0 + 16 * (n >> 2), npages), page_of(a, tab, tok0 + 16 * g, npages)};
+    }
+
+    // Block of 16 tokens of a page (a lane without a page reads the first
+    // page's codes, and masks them).
+    __device__ __forceinline__ static long block_of(const AttnParams& a, int id, int tok, int kvh) {
+        const int page = (unsigned)id < (unsigned)a.pages ? id : 0;
+        const long blocks = ((long)page * a.kv_heads + kvh) << (a.shift - 4);
+        return (blocks + ((tok & ((1 << a.shift) - 1)) >> 4)) * (16 * HD);
+    }
+
+    __device__ __forceinline__ static void load_k(const AttnParams& a, const Pages& pg, int tok0, int kvh, int n, int g,
+                                                  Codes& c) {
+        const int8_t* kp = a.k + block_of(a, pg.k, tok0 + 16 * (n >> 2), kvh) + 256 * g + 16 * (n & 3);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
-                if (HD >= 64 || 16 * g < HD) c.k[t][s] = ldg(kp + 4 * t * HD + 64 * s);
+                if (HD >= 64 || 16 * g < HD) c.k[t][s] = ldg(kp + 64 * t + 1024 * s);
                 else c.k[t][s] = v4i{0, 0, 0, 0};
             }
         }
-        const int8_t* vp = a.v + ((bv * HD + n) << a.shift) + (tv & mask);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) c.v[d] = ldg(vp + ((long)(16 * d) << a.shift));
     }
 
-    // Scores of a step, the running maximum and sum, and the value product.
-    __device__ __forceinline__ void step(const Codes& c, int tok0, int g, int limit, bool full) {
-        float x[16];
-        const float f = qf * c.ks;
+    __device__ __forceinline__ static void load_scales(const AttnParams& a, const Pages& pg, int kvh, Codes& c) {
+        c.ok = (unsigned)pg.v < (unsigned)a.pages;
+        const long bv = (long)(c.ok ? pg.v : 0) * a.kv_heads + kvh;
+        c.ks = a.ks[bv];
+        c.vs = a.vs[bv];
+        c.vs = c.ok ? c.vs : 0.0f;
+    }
+
+    __device__ __forceinline__ static void load_v(const AttnParams& a, const Pages& pg, int tok0, int kvh, int n, int g,
+                                                  Codes& c) {
+        const int8_t* vp = a.v + block_of(a, pg.v, tok0 + 16 * g, kvh) + 16 * n;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) c.v[d] = ldg(vp + 256 * d);
+    }
+
+    // Scores of a step (digits joined, without their scale).
+    __device__ __forceinline__ void scores(const Codes& c, float* x) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             v4i acc[QD];
@@ -286,30 +323,33 @@ struct Wave {
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float y = (float)acc[QD - 1][i];
-#pragma unroll
-                for (int d = QD - 2; d >= 0; --d) y = __builtin_fmaf(y, 256.0f, (float)acc[d][i]);
-                x[4 * t + i] = y * f;
+                // (a digit's sum is under 2^23 at head_dim 256: shifted by one it fits)
+                const float top = (float)(acc[QD - 1][i] * 256 + acc[QD - 2][i]);
+                x[4 * t + i] = QD == 3 ? __builtin_fmaf(top, 256.0f, (float)acc[0][i]) : top;
             }
         }
+    }
+
+    // The running maximum and sum of a step, and its probabilities in fp16
+    // (of lane n's column, tokens 8 h .. 8 h + 7 of this lane in hi[h], lo[h]).
+    __device__ __forceinline__ void softmax(float* x, float ks, float vs, bool ok, int tok0, int g, int limit, bool full,
+                                            v8h* ph, v8h* pl) {
+        const float f = qf * ks;  // never negative: a score's order is that of x within a lane
+        const int left = ok ? limit - (tok0 + 16 * g) : 0;
         if (!full) {
-            const int left = c.ok ? limit - (tok0 + 16 * g) : 0;
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] = i < left ? x[i] : kNegInf;
         }
         float mx = x[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
-        mx = fmaxf(mx, shfl_xor_f(mx, 16));
-        mx = fmaxf(mx, shfl_xor_f(mx, 32));
-        float vmax = fmaxf(c.vs, shfl_xor_f(c.vs, 16));
-        vmax = fmaxf(vmax, shfl_xor_f(vmax, 32));
-        const float m_new = fmaxf(m, mx);
-        const float base = m_new == kNegInf ? 0.0f : m_new;
-        // the values' scales count relative to the largest so far, as a power of two
-        float ref_new = ref;
-        if (vmax > ref) ref_new = __uint_as_float(((__float_as_uint(vmax) >> 23) + 1) << 23);
-        if (__any(m_new > m || ref_new > ref)) {
+        mx = column_max(mx * f);  // (no token: -inf, or NaN at f = 0, which the maximum leaves out)
+        const float vmax = column_max(vs);
+        if (__any(mx > m + kSlack || vmax > ref)) {
+            // the values' scales count relative to the largest so far, as a power of two
+            const float ref_new = vmax > ref ? __uint_as_float(((__float_as_uint(vmax) >> 23) + 1) << 23) : ref;
+            const float m_new = fmaxf(m, mx);
+            base = m_new == kNegInf ? 0.0f : m_new;
             const float al = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - base);
             l *= al;
             const float ao = al * (ref / ref_new);
@@ -317,30 +357,49 @@ struct Wave {
             for (int d = 0; d < ND; ++d) o[d] *= ao;
             m = m_new;
             ref = ref_new;
+            unit = kPeak / ref;
         }
-        const float pf = c.vs * (kPeak / ref);
+        const float pf = vs * unit;
         uint32_t hi[8], lo[8];
         float sum = 0.0f;
+        // (fused: a score keeps the bits that the product would round off)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(x[i], f, -base);
+        if (__any(fabsf(base) >= kHuge)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = fminf(x[i], kSlack);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float p0 = __builtin_amdgcn_exp2f(x[2 * i] - base), p1 = __builtin_amdgcn_exp2f(x[2 * i + 1] - base);
+            float p0 = __builtin_amdgcn_exp2f(x[2 * i]), p1 = __builtin_amdgcn_exp2f(x[2 * i + 1]);
+            if (!full) {
+                p0 = 2 * i < left ? p0 : 0.0f;
+                p1 = 2 * i + 1 < left ? p1 : 0.0f;
+            }
             sum += p0 + p1;
             const float w0 = p0 * pf, w1 = p1 * pf;
-            const v2h h = {(_Float16)w0, (_Float16)w1};
-            hi[i] = __builtin_bit_cast(uint32_t, h);
+            hi[i] = __builtin_bit_cast(uint32_t, v2h{(_Float16)w0, (_Float16)w1});
             if (PL == 2) {
-                const v2h r = {(_Float16)(w0 - (float)h[0]), (_Float16)(w1 - (float)h[1])};
+                // the remainder is taken from the packed bits themselves: the
+                // compiler may otherwise round the product to fp16 a second
+                // time, fused, and the two disagree at ties
+                asm("" : "+v"(hi[i]));
+                const v2h h = __builtin_bit_cast(v2h, hi[i]);
+                const v2h r = {(_Float16)__builtin_fmaf((float)h[0], -1.0f, w0), (_Float16)__builtin_fmaf((float)h[1], -1.0f, w1)};
                 lo[i] = __builtin_bit_cast(uint32_t, r);
             }
         }
         l += sum;
-        const v8h h0 = __builtin_bit_cast(v8h, v4i{(int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]});
-        const v8h h1 = __builtin_bit_cast(v8h, v4i{(int)hi[4], (int)hi[5], (int)hi[6], (int)hi[7]});
-        v8h l0, l1;
-        if (PL == 2) {
-            l0 = __builtin_bit_cast(v8h, v4i{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3]});
-            l1 = __builtin_bit_cast(v8h, v4i{(int)lo[4], (int)lo[5], (int)lo[6], (int)lo[7]});
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            ph[h] = __builtin_bit_cast(v8h, v4i{(int)hi[4 * h], (int)hi[4 * h + 1], (int)hi[4 * h + 2], (int)hi[4 * h + 3]});
+            if (PL == 2)
+                pl[h] = __builtin_bit_cast(v8h, v4i{(int)lo[4 * h], (int)lo[4 * h + 1], (int)lo[4 * h + 2], (int)lo[4 * h + 3]});
         }
+    }
+
+    // O^T += V^T P^T
+    __device__ __forceinline__ void values(const Codes& c, const v8h* ph, const v8h* pl) {
         const v2h bias = {(_Float16)1152.0f, (_Float16)1152.0f};
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
@@ -354,12 +413,11 @@ struct Wave {
                 w[j >> 1][2 * (j & 1)] = (int)__builtin_bit_cast(uint32_t, a);
                 w[j >> 1][2 * (j & 1) + 1] = (int)__builtin_bit_cast(uint32_t, b);
             }
-            const v8h v0 = __builtin_bit_cast(v8h, w[0]), v1 = __builtin_bit_cast(v8h, w[1]);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, h0, o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, h1, o[d], 0, 0, 0);
-            if (PL == 2) {
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, l0, o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, l1, o[d], 0, 0, 0);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const v8h v = __builtin_bit_cast(v8h, w[h]);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[h], o[d], 0, 0, 0);
+                if (PL == 2) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[h], o[d], 0, 0, 0);
             }
         }
     }
@@ -381,7 +439,8 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(AttnParams a) {
     const int n = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.y, part = blockIdx.z;
     int first_tile;
-    const int x = blockIdx.x;
+    // the last tiles of a chunk attend to the most: they start first
+    const int x = WSPLIT ? blockIdx.x : gridDim.x - 1 - blockIdx.x;
     const int r = find_request(a, CT, x, lane, &first_tile);
     if (r < 0) return;
     int start = a.row_start[r], end = a.row_start[r + 1];
@@ -422,20 +481,41 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(AttnParams a) {
     if (first < s1) {
         const int32_t* tab = a.table + (long)r * a.max_pages;
         const int npages = (most + (1 << a.shift) - 1) >> a.shift;
-        typename Wave<HD, QD, PL>::Codes c;
-        w.load_codes(a, tab, first * kStep, npages, kvh, n, g, c);
+        using W = Wave<HD, QD, PL>;
+        typename W::Codes c;
+        typename W::Pages pg = W::pages_of(a, tab, first * kStep, npages, n, g);
+        W::load_k(a, pg, first * kStep, kvh, n, g, c);
+        W::load_scales(a, pg, kvh, c);
+        W::load_v(a, pg, first * kStep, kvh, n, g, c);
+        pg = W::pages_of(a, tab, (first + stride) * kStep, npages, n, g);
         w.load_q(a, (long)row * a.q_stride + (long)head * HD, valid, g);
-        for (int s = first; s < s1; s += stride) {
-            const int tok0 = s * kStep;
-            const bool full = tok0 + kStep <= least && __all(c.ok);
-            w.step(c, tok0, g, limit, full);
-            if (s + stride < s1) w.load_codes(a, tab, (s + stride) * kStep, npages, kvh, n, g, c);
+        // the next step's keys are on their way from the end of this step's
+        // scores on, its values from the end of this step's product, its page
+        // numbers a step earlier
+        int s = first;
+        float x[16];
+        v8h ph[2], pl[2];
+        for (; s + stride < s1; s += stride) {
+            const int tok0 = s * kStep, tok1 = (s + stride) * kStep;
+            w.scores(c, x);
+            const float ks = c.ks, vs = c.vs;
+            const bool ok = c.ok;
+            const typename W::Pages now = pg;
+            W::load_k(a, now, tok1, kvh, n, g, c);
+            W::load_scales(a, now, kvh, c);
+            pg = W::pages_of(a, tab, tok1 + stride * kStep, npages, n, g);
+            w.softmax(x, ks, vs, ok, tok0, g, limit, tok0 + kStep <= least && __all(ok), ph, pl);
+            w.values(c, ph, pl);
+            W::load_v(a, now, tok1, kvh, n, g, c);
         }
+        w.scores(c, x);
+        w.softmax(x, c.ks, c.vs, c.ok, s * kStep, g, limit, s * kStep + kStep <= least && __all(c.ok), ph, pl);
+        w.values(c, ph, pl);
     }
     float l = w.l;
     l += shfl_xor_f(l, 16);
     l += shfl_xor_f(l, 32);
-    const float unit = w.ref * (1.0f / kPeak);
+    const float unit = w.ref / kPeak;
     float* part_o = a.part_o + ((long)part * a.rows * a.heads + rh) * HD;
     float* part_ml = a.part_ml + ((long)part * a.rows * a.heads + rh) * 2;
     if (WSPLIT) {

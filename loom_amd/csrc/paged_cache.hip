@@ -263,8 +263,9 @@ __device__ __forceinline__ float finite_abs(float x) {
 // sign of |x| - (c +- 1/2) s, one fused operation, is exact (s >= 2^-107).
 // NaN gives 0, an infinity the largest code.
 __device__ __forceinline__ int code_of(float x, float s, float inv) {
+    if (s == 0.0f) return 0;
     const float a = fabsf(x);
-    if (!(a <= kMaxFinite)) return (a != a || s == 0.0f) ? 0 : (x > 0 ? 127 : -127);
+    if (!(a <= kMaxFinite)) return a != a ? 0 : (x > 0 ? 127 : -127);
     float c = floorf(a * inv + 0.5f);
     if (__builtin_fmaf(-(c - 0.5f), s, a) < 0.0f) c -= 1.0f;
     else if (__builtin_fmaf(-(c + 0.5f), s, a) >= 0.0f) c += 1.0f;
@@ -285,92 +286,193 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
-// One wave per (run, head, side).  A run is the consecutive rows whose slots
-// follow one another within one page; the wave of a run's first row does all
-// of it, the others leave at once.  The page's scale is the larger of what it
-// had (unless the run starts the page: then nothing of it counts any more)
-// and the run's largest magnitude / 127.  When it grows, the codes of the
-// earlier tokens are rounded again at the new scale.
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void kv_append_kernel(KvPages c, const T* __restrict__ k, const T* __restrict__ v,
-                                                        int rows, long k_stride, long v_stride,
-                                                        const int32_t* __restrict__ slots) {
-    const int lane = threadIdx.x & 63;
-    const int row = blockIdx.x;
-    const int job = blockIdx.y * 4 + (threadIdx.x >> 6);
-    if (job >= 2 * c.kv_heads) return;
-    const int head = job >> 1;
-    const bool is_v = job & 1;
-    const int slot = slots[row];
-    if (slot < 0 || slot >= c.pages * c.page) return;
-    const int page = slot / c.page, off = slot % c.page;
-    if (row > 0 && off > 0 && slots[row - 1] == slot - 1) return;  // not a run's first row
-    int n = 0;  // tokens of the run
-    for (int base = 0; base < c.page; base += 64) {
-        const int t = base + lane;
-        const bool more = row + t < rows && off + t < c.page && slots[row + t] == slot + t;
-        const unsigned long long m = ~__ballot(more);
-        if (m) {
-            n = base + __builtin_ctzll(m);
-            break;
-        }
-        n = base + 64;
-    }
-    const T* src = (is_v ? v + (long)row * v_stride : k + (long)row * k_stride) + head * HD;
-    const long stride = is_v ? v_stride : k_stride;
-    float* scale_at = (is_v ? c.v_scale : c.k_scale) + (long)page * c.kv_heads + head;
-    float big = 0.0f;
-    // HD is a power of two: a wave reads 64 consecutive values of a row, or
-    // several rows where one has fewer
-    for (int i = lane; i < n * HD; i += 64) big = fmaxf(big, finite_abs(as_f32<T>(src[(long)(i / HD) * stride + i % HD])));
-    big = wave_max(big);
-    const float from = off == 0 ? 0.0f : *scale_at;
-    const float own = big < kTinyAmax ? 0.0f : big / 127.0f;
-    const float to = fmaxf(from, own);
-    const float inv = to > 0.0f ? 1.0f / to : 0.0f;
-    const bool grows = off > 0 && to > from;
-    int8_t* codes = (is_v ? c.v : c.k) + ((long)page * c.kv_heads + head) * (long)(c.page * HD);
-    if (!is_v) {
-        if (grows) {
-            for (int i = lane; i < off * HD; i += 64) codes[i] = (int8_t)recode(codes[i], from, to);
-        }
-        for (int i = lane; i < n * HD; i += 64) {
-            const float x = as_f32<T>(src[(long)(i / HD) * stride + i % HD]);
-            codes[off * HD + i] = (int8_t)(to > 0.0f ? code_of(x, to, inv) : 0);
+// Four consecutive elements (vec: one load).
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, bool vec, float* x) {
+    if (vec) {
+        if (sizeof(T) == 4) {
+            const float4 f = *(const float4*)p;
+            x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+        } else {
+            const uint2 u = *(const uint2*)p;
+            x[0] = __uint_as_float(u.x << 16), x[1] = __uint_as_float(u.x & 0xffff0000u);
+            x[2] = __uint_as_float(u.y << 16), x[3] = __uint_as_float(u.y & 0xffff0000u);
         }
     } else {
-        // four tokens of one dimension are one word
-        const int q0 = grows ? 0 : off >> 2, q1 = (off + n + 3) >> 2;
-        for (int i = lane; i < (q1 - q0) * HD; i += 64) {
-            const int d = i % HD, q = q0 + i / HD;
-            uint32_t* at = (uint32_t*)(codes + (long)d * c.page + 4 * q);
-            const bool whole = 4 * q >= off && 4 * q + 4 <= off + n;
-            uint32_t w = whole ? 0u : *at;
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const int t = 4 * q + b - off;
-                int code = (int8_t)(w >> (8 * b));
-                if (t < 0) {
-                    if (grows) code = recode(code, from, to);
-                } else if (t < n) {
-                    code = to > 0.0f ? code_of(as_f32<T>(src[(long)t * stride + d]), to, inv) : 0;
-                }
-                w = (w & ~(0xffu << (8 * b))) | ((uint32_t)(uint8_t)code << (8 * b));
+        for (int i = 0; i < 4; ++i) x[i] = as_f32<T>(p[i]);
+    }
+}
+
+constexpr int kWindow = 16;  // rows whose runs one workgroup looks for
+
+// Jobs are (run, head, side), a wave each.  A run is the consecutive rows
+// whose slots follow one another within one page, and belongs to the window
+// of its first row.  The page's scale is the larger of what it had (unless the
+// run starts the page: then nothing of it counts any more) and the run's
+// largest magnitude / 127.  When it grows, the codes of the earlier tokens are
+// rounded again at the new scale.
+//
+// Bound by memory (one read of the rows, one write of the codes): a lane takes
+// four dimensions of a token (keys), or of four tokens (values, whose codes
+// lie token by token), in one load each, and keeps up to 2048 values of a run
+// in registers between the search for the largest and the rounding.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void kv_append_kernel(KvPages c, const T* __restrict__ k, const T* __restrict__ v,
+                                                        int rows, long k_stride, long v_stride, bool vec,
+                                                        const int32_t* __restrict__ slots) {
+    constexpr int D4 = HD / 4;
+    const int lane = threadIdx.x & 63;
+    const int row0 = blockIdx.x * kWindow;
+    // rows of the window that start a run
+    bool leads = false;
+    if (lane < kWindow && row0 + lane < rows) {
+        const int row = row0 + lane, slot = slots[row];
+        leads = slot >= 0 && slot < c.pages * c.page && !(row > 0 && slot % c.page > 0 && slots[row - 1] == slot - 1);
+    }
+    unsigned long long left = __ballot(leads);
+    const int sides = 2 * c.kv_heads, waves = gridDim.y * 4;
+    int job = blockIdx.y * 4 + (threadIdx.x >> 6);
+    for (; left; left &= left - 1, job -= sides) {
+        if (job >= sides) continue;  // (of a later run)
+        const int row = row0 + __builtin_ctzll(left);
+        const int slot = slots[row];
+        const int page = slot / c.page, off = slot % c.page;
+        int n = 0;  // tokens of the run
+        for (int base = 0; base < c.page; base += 64) {
+            const int t = base + lane;
+            const bool more = row + t < rows && off + t < c.page && slots[row + t] == slot + t;
+            const unsigned long long m = ~__ballot(more);
+            if (m) {
+                n = base + __builtin_ctzll(m);
+                break;
             }
-            *at = w;
+            n = base + 64;
+        }
+        for (; job < sides; job += waves) {
+            const int head = job >> 1;
+            const bool is_v = job & 1;
+            const long stride = is_v ? v_stride : k_stride;
+            const T* src = (is_v ? v : k) + (long)row * stride + head * HD;
+            float* scale_at = (is_v ? c.v_scale : c.k_scale) + (long)page * c.kv_heads + head;
+            int8_t* codes = (is_v ? c.v : c.k) + ((long)page * c.kv_heads + head) * (long)(c.page * HD);
+            const float had = off == 0 ? 0.0f : *scale_at;
+            float x[8][4];
+            float big = 0.0f;
+            // keys: unit u is dimensions 4 (u % D4) .. of token u / D4
+            // values: unit u is four tokens of the same, quad by quad
+            const int q0 = off >> 2, quads = ((off + n + 3) >> 2) - q0;
+            const int units = is_v ? quads * D4 : n * D4;
+            const int per = is_v ? 2 : 8;  // units in registers
+            auto fetch = [&](int u0) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    int t, d;
+                    bool in;
+                    if (is_v) {
+                        const int u = u0 + lane + 64 * (i >> 2);
+                        d = 4 * (u % D4);
+                        t = 4 * (q0 + u / D4) + (i & 3) - off;
+                        in = u < units && t >= 0 && t < n;
+                    } else {
+                        const int u = u0 + lane + 64 * i;
+                        d = 4 * (u % D4);
+                        t = u / D4;
+                        in = u < units;
+                    }
+                    if (in) load4<T>(src + (long)t * stride + d, vec, x[i]);
+                    else x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
+                }
+            };
+            for (int u0 = 0; u0 < units; u0 += 64 * per) {
+                fetch(u0);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) big = fmaxf(big, finite_abs(x[i][j]));
+                }
+            }
+            big = wave_max(big);
+            const float own = big < kTinyAmax ? 0.0f : big / 127.0f;
+            const float to = fmaxf(had, own);
+            const float inv = to > 0.0f ? 1.0f / to : 0.0f;
+            const bool grows = off > 0 && to > had;
+            if (grows) {
+                if (is_v) {  // whole words of earlier tokens (a word shared with the run is done below)
+                    for (int i = lane; i < q0 * HD; i += 64) {
+                        uint32_t* at = (uint32_t*)(codes + v_offset(4 * (i / HD), i % HD, HD));
+                        uint32_t w = *at, z = 0;
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) z |= (uint32_t)(uint8_t)recode((int8_t)(w >> (8 * b)), had, to) << (8 * b);
+                        *at = z;
+                    }
+                } else {
+                    for (int i = lane; i < off * D4; i += 64) {
+                        uint32_t* at = (uint32_t*)(codes + k_offset(i / D4, 4 * (i % D4), HD));
+                        uint32_t w = *at, z = 0;
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) z |= (uint32_t)(uint8_t)recode((int8_t)(w >> (8 * b)), had, to) << (8 * b);
+                        *at = z;
+                    }
+                }
+            }
+            for (int u0 = 0; u0 < units; u0 += 64 * per) {
+                if (units > 64 * per) fetch(u0);
+                if (is_v) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int u = u0 + lane + 64 * i;
+                        if (u >= units) continue;
+                        const int q = q0 + u / D4;
+                        const int t0 = 4 * q - off;
+                        const bool whole = t0 >= 0 && t0 + 4 <= n;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t* at = (uint32_t*)(codes + v_offset(4 * q, 4 * (u % D4) + j, HD));
+                            uint32_t w = whole ? 0u : *at, z = 0;
+#pragma unroll
+                            for (int b = 0; b < 4; ++b) {
+                                int code = (int8_t)(w >> (8 * b));
+                                if (t0 + b < 0) {
+                                    if (grows) code = recode(code, had, to);
+                                } else if (t0 + b < n) {
+                                    code = code_of(x[4 * i + b][j], to, inv);
+                                }
+                                z |= (uint32_t)(uint8_t)code << (8 * b);
+                            }
+                            *at = z;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int u = u0 + lane + 64 * i;
+                        if (u >= units) continue;
+                        uint32_t z = 0;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) z |= (uint32_t)(uint8_t)code_of(x[i][j], to, inv) << (8 * j);
+                        *(uint32_t*)(codes + k_offset(off + u / D4, 4 * (u % D4), HD)) = z;
+                    }
+                }
+            }
+            if (lane == 0) *scale_at = to;
         }
     }
-    if (lane == 0) *scale_at = to;
 }
 
 template <typename T>
 static hipError_t append_typed(const KvPages& c, const void* k, const void* v, int rows, long ks, long vs,
                                const int32_t* slots, hipStream_t s) {
-    const dim3 grid((unsigned)rows, (unsigned)ceil_div(2 * c.kv_heads, 4));
-#define APPEND(HD)                                                                                                \
-    case HD:                                                                                                      \
+    const uintptr_t m = 4 * sizeof(T) - 1;
+    const bool vec = (((uintptr_t)k | (uintptr_t)v) & m) == 0 && ((ks | vs) & 3) == 0;
+    // few rows: a wave for every job there may be; many: runs of several rows
+    // are likely, and waves go on to further runs where there are more
+    const int jobs = 2 * c.kv_heads * (rows < 1024 ? (rows < kWindow ? rows : kWindow) : 1);
+    const dim3 grid((unsigned)ceil_div(rows, kWindow), (unsigned)(jobs < 4 * 65535 ? ceil_div(jobs, 4) : 65535));
+#define APPEND(HD)                                                                                               \
+    case HD:                                                                                                     \
         hipLaunchKernelGGL((kv_append_kernel<T, HD>), grid, dim3(256), 0, s, c, (const T*)k, (const T*)v, rows, ks, \
-                           vs, slots);                                                                            \
+                           vs, vec, slots);                                                                      \
         break;
     switch (c.hd) {
         APPEND(32)
@@ -389,25 +491,51 @@ hipError_t launch_kv_append(const KvPages& c, const void* k, const void* v, int 
                             : append_typed<float>(c, k, v, rows, k_stride, v_stride, slots, s);
 }
 
-// Values code * scale of given slots; no slot reads as zeros.
-__global__ __launch_bounds__(256) void kv_read_kernel(KvPages c, const int32_t* __restrict__ slots,
+// Values code * scale of given slots; no slot reads as zeros.  A workgroup
+// takes 16 rows of one head: the codes of values, whose tokens lie side by
+// side, are read with the rows on neighbouring lanes (rows of one page share
+// their lines) and turned in LDS, so that both sides are written in whole lines.
+__global__ __launch_bounds__(256) void kv_read_kernel(KvPages c, const int32_t* __restrict__ slots, int rows,
                                                       float* __restrict__ k, float* __restrict__ v) {
-    const int row = blockIdx.x;
-    const int slot = slots[row];
-    const bool in = slot >= 0 && slot < c.pages * c.page;
-    const int page = in ? slot / c.page : 0, off = in ? slot % c.page : 0;
-    for (int i = threadIdx.x; i < c.kv_heads * c.hd; i += blockDim.x) {
-        const int h = i / c.hd, d = i % c.hd;
+    __shared__ int8_t turn[256 * 17];
+    const int row0 = blockIdx.x * 16, h = blockIdx.y;
+    const int t = threadIdx.x;
+    {
+        const int row = row0 + (t & 15);
+        const int slot = row < rows ? slots[row] : -1;
+        const bool in = slot >= 0 && slot < c.pages * c.page;
+        const int page = in ? slot / c.page : 0, off = in ? slot % c.page : 0;
+        const int8_t* src = c.v + ((long)page * c.kv_heads + h) * ((long)c.page * c.hd) + v_offset(off, 0, c.hd);
+#pragma unroll 4
+        for (int d = t >> 4; d < c.hd; d += 16) turn[d * 17 + (t & 15)] = in ? src[16 * d] : (int8_t)0;
+    }
+    __syncthreads();
+    const int d4 = c.hd >> 2;
+    for (int i = t; i < 16 * d4; i += 256) {
+        const int rr = i / d4, d = 4 * (i % d4), row = row0 + rr;
+        if (row >= rows) break;
+        const int slot = slots[row];
+        const bool in = slot >= 0 && slot < c.pages * c.page;
+        const int page = in ? slot / c.page : 0, off = in ? slot % c.page : 0;
         const long ph = (long)page * c.kv_heads + h;
-        const long block = ph * ((long)c.page * c.hd);
-        const long at = (long)row * c.kv_heads * c.hd + i;
-        k[at] = in ? (float)c.k[block + (long)off * c.hd + d] * c.k_scale[ph] : 0.0f;
-        v[at] = in ? (float)c.v[block + (long)d * c.page + off] * c.v_scale[ph] : 0.0f;
+        const float fk = in ? c.k_scale[ph] : 0.0f, fv = in ? c.v_scale[ph] : 0.0f;
+        uint32_t w = 0;
+        if (in) w = *(const uint32_t*)(c.k + ph * ((long)c.page * c.hd) + k_offset(off, d, c.hd));
+        const long at = ((long)row * c.kv_heads + h) * c.hd + d;
+        float a[4], b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            a[j] = in ? (float)(int8_t)(w >> (8 * j)) * fk : 0.0f;
+            b[j] = in ? (float)turn[(d + j) * 17 + rr] * fv : 0.0f;
+        }
+        *(float4*)(k + at) = make_float4(a[0], a[1], a[2], a[3]);
+        *(float4*)(v + at) = make_float4(b[0], b[1], b[2], b[3]);
     }
 }
 
 hipError_t launch_kv_read(const KvPages& c, const int32_t* slots, int rows, float* k, float* v, hipStream_t s) {
-    hipLaunchKernelGGL(kv_read_kernel, dim3((unsigned)rows), dim3(256), 0, s, c, slots, k, v);
+    hipLaunchKernelGGL(kv_read_kernel, dim3((unsigned)ceil_div(rows, 16), (unsigned)c.kv_heads), dim3(256), 0, s, c, slots,
+                       rows, k, v);
     return hipGetLastError();
 }
 

@@ -188,50 +188,70 @@ class PageTable:
 
 class PagedCache:
     """Keys and values of one layer as int8 codes in pages, with an fp32 scale
-    for each page, head and side (value = code * scale):
+    for each page, head and side (value = code * scale).  2 bytes per cached key
+    and value where the fp32 ring takes 8.
 
-        k [num_pages, kv_heads, page_size, head_dim]   k_scale [num_pages, kv_heads]
-        v [num_pages, kv_heads, head_dim, page_size]   v_scale [num_pages, kv_heads]
+    The codes lie in blocks of 16 tokens, in the order of attention's matrix
+    operands:
 
-    2 bytes per cached value pair where the fp32 ring takes 8."""
+        k [num_pages, kv_heads, page_size / 16, head_dim / 16, 16 tokens, 16]
+        v [num_pages, kv_heads, page_size / 16, head_dim, 16 tokens]
+        k_scale, v_scale [num_pages, kv_heads]
+
+    ``from_tensors`` and ``codes`` convert from and to plain order."""
 
     def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, device=0):
         torch = _torch()
-        dev = f"cuda:{_index(device)}"
-        self._set(torch.zeros(num_pages, kv_heads, page_size, head_dim, dtype=torch.int8, device=dev),
-                  torch.zeros(num_pages, kv_heads, head_dim, page_size, dtype=torch.int8, device=dev),
-                  torch.zeros(num_pages, kv_heads, dtype=torch.float32, device=dev),
-                  torch.zeros(num_pages, kv_heads, dtype=torch.float32, device=dev))
+        self._shape(num_pages, page_size, kv_heads, head_dim, _index(device))
+        kw = dict(device=f"cuda:{self.device}")
+        b = page_size // 16
+        self._hold(torch.zeros(num_pages, kv_heads, b, head_dim // 16, 16, 16, dtype=torch.int8, **kw),
+                   torch.zeros(num_pages, kv_heads, b, head_dim, 16, dtype=torch.int8, **kw),
+                   torch.zeros(num_pages, kv_heads, dtype=torch.float32, **kw),
+                   torch.zeros(num_pages, kv_heads, dtype=torch.float32, **kw))
 
     @classmethod
     def from_tensors(cls, k, v, k_scale, v_scale) -> "PagedCache":
-        """A cache over tensors of the caller, in the layout above."""
-        self = cls.__new__(cls)
-        self._set(k, v, k_scale, v_scale)
-        return self
-
-    def _set(self, k, v, k_scale, v_scale) -> None:
+        """A cache that holds these codes and scales: k int8 [num_pages,
+        kv_heads, page_size, head_dim], v int8 [num_pages, kv_heads, head_dim,
+        page_size], scales float32 [num_pages, kv_heads].  They are copied."""
         torch = _torch()
         if k.dim() != 4:
             raise ValueError("k must be [num_pages, kv_heads, page_size, head_dim]")
         pages, heads, page, hd = k.shape
+        self = cls.__new__(cls)
+        dev = _device_of(k, "k")
+        self._shape(pages, page, heads, hd, dev)
+        _want(k, torch.int8, None, dev, "k")
+        _want(v, torch.int8, (pages, heads, hd, page), dev, "v")
+        _want(k_scale, torch.float32, (pages, heads), dev, "k_scale")
+        _want(v_scale, torch.float32, (pages, heads), dev, "v_scale")
+        fmt = torch.contiguous_format
+        self._hold(k.view(pages, heads, page // 16, 16, hd // 16, 16).permute(0, 1, 2, 4, 3, 5).clone(memory_format=fmt),
+                   v.view(pages, heads, hd, page // 16, 16).permute(0, 1, 3, 2, 4).clone(memory_format=fmt),
+                   k_scale.clone(), v_scale.clone())
+        return self
+
+    def codes(self):
+        """(k, v): copies of the codes, both int8 [num_pages, kv_heads,
+        page_size, head_dim]."""
+        shape = (self.num_pages, self.kv_heads, self.page_size, self.head_dim)
+        return (self.k.permute(0, 1, 2, 4, 3, 5).reshape(shape), self.v.transpose(3, 4).reshape(shape))
+
+    def _shape(self, pages: int, page: int, heads: int, hd: int, dev: int) -> None:
         if page not in PAGE_SIZES:
             raise ValueError(f"page_size must be one of {PAGE_SIZES}")
         if hd not in HEAD_DIMS:
             raise ValueError(f"head_dim must be one of {HEAD_DIMS}")
         if pages <= 0 or heads <= 0 or pages * page > 2 ** 31 - 1:
             raise ValueError("a cache holds 1 to 2^31 - 1 tokens of at least one head")
-        dev = _device_of(k, "k")
-        ptrs = [_want(k, torch.int8, None, dev, "k"),
-                _want(v, torch.int8, (pages, heads, hd, page), dev, "v"),
-                _want(k_scale, torch.float32, (pages, heads), dev, "k_scale"),
-                _want(v_scale, torch.float32, (pages, heads), dev, "v_scale")]
-        if ptrs[0] % 16 or ptrs[1] % 16:
-            raise ValueError("k and v must be 16-byte aligned")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, page, hd
         self.device = dev
-        self._c = _lib.KvPages(*ptrs, pages, page, heads, hd)
+
+    def _hold(self, k, v, k_scale, v_scale) -> None:
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._c = _lib.KvPages(*(t.data_ptr() for t in (k, v, k_scale, v_scale)), self.num_pages, self.page_size,
+                               self.kv_heads, self.head_dim)
         self._p = C.byref(self._c)
 
     def append(self, k, v, slots) -> None:

@@ -111,8 +111,7 @@ def new_cache(paged, pages, page, heads, hd, seed):
 
 
 def snapshot(c):
-    return (c.k.cpu().numpy().astype(np.float64), c.v.cpu().numpy().transpose(0, 1, 3, 2).astype(np.float64),
-            c.k_scale.cpu().numpy(), c.v_scale.cpu().numpy())
+    return (*(t.cpu().numpy().astype(np.float64) for t in c.codes()), c.k_scale.cpu().numpy(), c.v_scale.cpu().numpy())
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -226,7 +225,8 @@ def run_attention(paged, hd, kv, group, page, dtype, ctx, new, seed=0, pad=0, sl
     got = paged.attention(dq, c, ints(table), ints(start), ints(pos), out=out, max_context=max_context)
     assert got is out
     scale = hd ** -0.5
-    kc, vc = c.k.cpu().numpy(), c.v.cpu().numpy()
+    kc, vc = (t.cpu().numpy() for t in c.codes())
+    vc = vc.transpose(0, 1, 3, 2)
     ks, vs = c.k_scale.cpu().numpy(), c.v_scale.cpu().numpy()
     qn = q.double().numpy()
     want = ref.attention(qn, kc, vc, ks, vs, table, start, pos, scale)
@@ -275,6 +275,20 @@ def test_attention_finds_requests(paged, requests):
     new = r.integers(0, 2, requests)
     new[-1] = 1
     run_attention(paged, 32, 1, 2, 16, torch.float32, np.maximum(new, r.integers(1, 20, requests)), new)
+
+
+def test_codes_in_and_out(paged):
+    g = torch.Generator(device="cuda").manual_seed(0)
+    for pages, heads, page, hd in ((3, 2, 16, 32), (2, 1, 128, 64), (1, 3, 32, 256)):
+        k = torch.randint(-127, 128, (pages, heads, page, hd), generator=g, device="cuda").to(torch.int8)
+        v = torch.randint(-127, 128, (pages, heads, hd, page), generator=g, device="cuda").to(torch.int8)
+        ks, vs = (torch.rand(pages, heads, generator=g, device="cuda") for _ in range(2))
+        c = paged.PagedCache.from_tensors(k, v, ks, vs)
+        kc, vc = c.codes()
+        assert torch.equal(kc, k) and torch.equal(vc, v.transpose(2, 3))
+        a, b = c.read(torch.arange(pages * page, dtype=torch.int32, device="cuda"))
+        assert torch.equal(a, (k.float() * ks[:, :, None, None]).transpose(1, 2).reshape(pages * page, heads, hd))
+        assert torch.equal(b, (v.float() * vs[:, :, None, None]).permute(0, 3, 1, 2).reshape(pages * page, heads, hd))
 
 
 def test_attention_float64_rows(paged):
