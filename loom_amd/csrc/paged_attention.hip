@@ -54,7 +54,7 @@ struct AttnParams {
     int32_t* active;  // [row][head]: parts of this row's context
     int pages, shift, kv_heads, max_pages, requests, rows, heads, group, splits, type, max_context;
     int min_steps;       // steps of a part
-    int lo_cols, hi_cols;  // this launch takes requests with lo_cols <= columns <= hi_cols
+    int hi_cols;  // requests of up to so many columns go to the rows kernel, others to the chunk kernel
     long q_stride, out_stride;
     float scale2;  // scale * log2(e)
     bool vec;      // rows of q and out are 16-byte aligned
@@ -67,6 +67,13 @@ __device__ __forceinline__ float column_max(float v) {
     v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ __forceinline__ float column_sum(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 __device__ __forceinline__ float shfl_xor_f(float v, int m) { return __shfl_xor(v, m, 64); }
@@ -170,6 +177,7 @@ __device__ __forceinline__ int find_request(const AttnParams& a, int ct, int x, 
     }
 }
 
+// 16 columns of one wave.
 template <int HD, int QD, int PL>
 struct Wave {
     static constexpr int NS = HD >= 64 ? HD / 64 : 1;  // 64-dimension steps of the score product
@@ -200,11 +208,8 @@ struct Wave {
                 big = fmaxf(big, fabsf(x[s][i]));
             }
         }
-        big = fmaxf(big, shfl_xor_f(big, 16));
-        big = fmaxf(big, shfl_xor_f(big, 32));
-        float nan = bad ? __builtin_nanf("") : 0.0f;
-        nan += shfl_xor_f(nan, 16);
-        nan += shfl_xor_f(nan, 32);
+        big = column_max(big);
+        const float nan = column_sum(bad ? __builtin_nanf("") : 0.0f);
         // largest fixed-point value: just under the digits' own, 127 * (1 + 256 (+ 65536))
         constexpr float kTop = QD == 3 ? 8355000.0f : 32600.0f;
         const bool zero = big < 0x1p-100f;
@@ -215,20 +220,20 @@ struct Wave {
         for (int s = 0; s < NS; ++s) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                uint32_t t[4];
+                uint32_t y[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float f = rintf(x[s][4 * w + i] * inv);
-                    f = fminf(fmaxf(f, -kTop), kTop);  // (NaN, infinities: any digits, qf is NaN)
-                    t[i] = ((uint32_t)(int)f + 0x80808080u) ^ 0x80808080u;  // signed digits, lowest byte first
+                    f = fminf(fmaxf(f, -kTop), kTop);  // (NaN, infinities: any digits, the sum is NaN)
+                    y[i] = ((uint32_t)(int)f + 0x80808080u) ^ 0x80808080u;  // signed digits, lowest byte first
                 }
-                const uint32_t a01 = __builtin_amdgcn_perm(t[1], t[0], 0x05010400u);
-                const uint32_t a23 = __builtin_amdgcn_perm(t[3], t[2], 0x05010400u);
+                const uint32_t a01 = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u);
+                const uint32_t a23 = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
                 qd[0][s][w] = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100u);
                 qd[1][s][w] = (int)__builtin_amdgcn_perm(a23, a01, 0x07060302u);
                 if (QD == 3) {
-                    const uint32_t b01 = __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0602u);
-                    const uint32_t b23 = __builtin_amdgcn_perm(t[3], t[2], 0x0c0c0602u);
+                    const uint32_t b01 = __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0602u);
+                    const uint32_t b23 = __builtin_amdgcn_perm(y[3], y[2], 0x0c0c0602u);
                     qd[QD - 1][s][w] = (int)__builtin_amdgcn_perm(b23, b01, 0x05040100u);
                 }
             }
@@ -245,106 +250,44 @@ struct Wave {
         unit = kPeak / ref;
     }
 
-    __device__ __forceinline__ static v4i ldg(const int8_t* p) { return *(const v4i*)p; }
-
-    // Codes of one step, the scales of this lane's page, and whether it has one.
-    struct Codes {
-        v4i k[4][NS];
-        v4i v[ND];
-        float ks, vs;
-        bool ok;
-    };
-    // Pages of this lane's key row and of its 16 tokens (-1: none).
-    struct Pages {
-        int k, v;
-    };
-
-    // (always a load, of the last page's number where tok is past it: a branch
-    // here would make the loop wait for every load it has under way)
-    __device__ __forceinline__ static int page_of(const AttnParams& a, const int32_t* tab, int tok, int npages) {
-        const unsigned i = (unsigned)tok >> a.shift;
-        const int id = tab[min(i, (unsigned)npages - 1)];
-        return i < (unsigned)npages ? id : -1;
-    }
-
-    __device__ __forceinline__ static Pages pages_of(const AttnParams& a, const int32_t* tab, int tok0, int npages, int n,
-                                                     int g) {
-        return Pages{page_of(a, tab, tok0 + 16 * (n >> 2), npages), page_of(a, tab, tok0 + 16 * g, npages)};
-    }
-
-    // Block of 16 tokens of a page (a lane without a page reads the first
-    // page's codes, and masks them).
-    __device__ __forceinline__ static long block_of(const AttnParams& a, int id, int tok, int kvh) {
-        const int page = (unsigned)id < (unsigned)a.pages ? id : 0;
-        const long blocks = ((long)page * a.kv_heads + kvh) << (a.shift - 4);
-        return (blocks + ((tok & ((1 << a.shift) - 1)) >> 4)) * (16 * HD);
-    }
-
-    __device__ __forceinline__ static void load_k(const AttnParams& a, const Pages& pg, int tok0, int kvh, int n, int g,
-                                                  Codes& c) {
-        const int8_t* kp = a.k + block_of(a, pg.k, tok0 + 16 * (n >> 2), kvh) + 256 * g + 16 * (n & 3);
+    // Scores of tile t (digits joined, without their scale): keys in rows.
+    __device__ __forceinline__ void tile(const v4i* k, float* x) const {
+        v4i acc[QD];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int d = 0; d < QD; ++d) acc[d] = v4i{0, 0, 0, 0};
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                if (HD >= 64 || 16 * g < HD) c.k[t][s] = ldg(kp + 64 * t + 1024 * s);
-                else c.k[t][s] = v4i{0, 0, 0, 0};
-            }
+        for (int s = 0; s < NS; ++s) {
+#pragma unroll
+            for (int d = 0; d < QD; ++d) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[s], qd[d][s], acc[d], 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            // (a digit's sum is at most 2^22 at head_dim 256: 256 times that fits)
+            const float top = (float)(acc[QD - 1][i] * 256 + acc[QD - 2][i]);
+            x[i] = QD == 3 ? __builtin_fmaf(top, 256.0f, (float)acc[0][i]) : top;
         }
     }
 
-    __device__ __forceinline__ static void load_scales(const AttnParams& a, const Pages& pg, int kvh, Codes& c) {
-        c.ok = (unsigned)pg.v < (unsigned)a.pages;
-        const long bv = (long)(c.ok ? pg.v : 0) * a.kv_heads + kvh;
-        c.ks = a.ks[bv];
-        c.vs = a.vs[bv];
-        c.vs = c.ok ? c.vs : 0.0f;
-    }
-
-    __device__ __forceinline__ static void load_v(const AttnParams& a, const Pages& pg, int tok0, int kvh, int n, int g,
-                                                  Codes& c) {
-        const int8_t* vp = a.v + block_of(a, pg.v, tok0 + 16 * g, kvh) + 16 * n;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) c.v[d] = ldg(vp + 256 * d);
-    }
-
-    // Scores of a step (digits joined, without their scale).
-    __device__ __forceinline__ void scores(const Codes& c, float* x) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            v4i acc[QD];
-#pragma unroll
-            for (int d = 0; d < QD; ++d) acc[d] = v4i{0, 0, 0, 0};
-#pragma unroll
-            for (int s = 0; s < NS; ++s) {
-#pragma unroll
-                for (int d = 0; d < QD; ++d)
-                    acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(c.k[t][s], qd[d][s], acc[d], 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // (a digit's sum is under 2^23 at head_dim 256: shifted by one it fits)
-                const float top = (float)(acc[QD - 1][i] * 256 + acc[QD - 2][i]);
-                x[4 * t + i] = QD == 3 ? __builtin_fmaf(top, 256.0f, (float)acc[0][i]) : top;
-            }
-        }
-    }
-
-    // The running maximum and sum of a step, and its probabilities in fp16
-    // (of lane n's column, tokens 8 h .. 8 h + 7 of this lane in hi[h], lo[h]).
-    __device__ __forceinline__ void softmax(float* x, float ks, float vs, bool ok, int tok0, int g, int limit, bool full,
+    // The running maximum and sum over the 16 scores x of this lane, four of
+    // each tile t, and their probabilities in fp16: 8 h .. 8 h + 7 in ph[h] (and
+    // pl[h]).  f[t], vs[t]: factors of tile t's scores and values; keep(i): score
+    // i counts (asked only when not `full`).
+    template <typename Keep>
+    __device__ __forceinline__ void softmax(float* x, const float* f, const float* vs, float vmax, bool full, Keep keep,
                                             v8h* ph, v8h* pl) {
-        const float f = qf * ks;  // never negative: a score's order is that of x within a lane
-        const int left = ok ? limit - (tok0 + 16 * g) : 0;
         if (!full) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = i < left ? x[i] : kNegInf;
+            for (int i = 0; i < 16; ++i) x[i] = keep(i) ? x[i] : kNegInf;
         }
-        float mx = x[0];
+        // (factors are never negative: a tile's largest score is that of its
+        // largest x; no token gives -inf, or NaN at a factor of 0, which the
+        // maximum leaves out)
+        float mx = kNegInf;
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
-        mx = column_max(mx * f);  // (no token: -inf, or NaN at f = 0, which the maximum leaves out)
-        const float vmax = column_max(vs);
+        for (int t = 0; t < 4; ++t) {
+            mx = fmaxf(mx, fmaxf(fmaxf(x[4 * t], x[4 * t + 1]), fmaxf(x[4 * t + 2], x[4 * t + 3])) * f[t]);
+        }
+        mx = column_max(mx);
         if (__any(mx > m + kSlack || vmax > ref)) {
             // the values' scales count relative to the largest so far, as a power of two
             const float ref_new = vmax > ref ? __uint_as_float(((__float_as_uint(vmax) >> 23) + 1) << 23) : ref;
@@ -359,22 +302,22 @@ struct Wave {
             ref = ref_new;
             unit = kPeak / ref;
         }
-        const float pf = vs * unit;
-        uint32_t hi[8], lo[8];
-        float sum = 0.0f;
         // (fused: a score keeps the bits that the product would round off)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(x[i], f, -base);
+        for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(x[i], f[i >> 2], -base);
         if (__any(fabsf(base) >= kHuge)) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] = fminf(x[i], kSlack);
         }
+        uint32_t hi[8], lo[8];
+        float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
+            const float pf = vs[i >> 1] * unit;
             float p0 = __builtin_amdgcn_exp2f(x[2 * i]), p1 = __builtin_amdgcn_exp2f(x[2 * i + 1]);
             if (!full) {
-                p0 = 2 * i < left ? p0 : 0.0f;
-                p1 = 2 * i + 1 < left ? p1 : 0.0f;
+                p0 = keep(2 * i) ? p0 : 0.0f;
+                p1 = keep(2 * i + 1) ? p1 : 0.0f;
             }
             sum += p0 + p1;
             const float w0 = p0 * pf, w1 = p1 * pf;
@@ -398,27 +341,72 @@ struct Wave {
         }
     }
 
-    // O^T += V^T P^T
-    __device__ __forceinline__ void values(const Codes& c, const v8h* ph, const v8h* pl) {
-        const v2h bias = {(_Float16)1152.0f, (_Float16)1152.0f};
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            // code + 128 as the low bits of an fp16 of 1024, less 1152
-            v4i w[2];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t u = (uint32_t)c.v[d][j] ^ 0x80808080u;
-                const v2h a = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias;
-                const v2h b = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias;
-                w[j >> 1][2 * (j & 1)] = (int)__builtin_bit_cast(uint32_t, a);
-                w[j >> 1][2 * (j & 1) + 1] = (int)__builtin_bit_cast(uint32_t, b);
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const v8h v = __builtin_bit_cast(v8h, w[h]);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[h], o[d], 0, 0, 0);
-                if (PL == 2) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[h], o[d], 0, 0, 0);
-            }
+    // O^T += V^T P^T of one 16-dimension tile and half of the step's tokens
+    __device__ __forceinline__ void value(int d, v8h v, v8h ph, v8h pl) {
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, o[d], 0, 0, 0);
+        if (PL == 2) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[d], 0, 0, 0);
+    }
+};
+
+// Four codes as fp16: code + 128 as the low bits of 1024, less 1152.
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t* out) {
+    const v2h bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+    const uint32_t u = w ^ 0x80808080u;
+    out[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias);
+    out[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias);
+}
+
+__device__ __forceinline__ v4i ldg(const int8_t* p) { return *(const v4i*)p; }
+
+// Page number of the 16 tokens at tok as the table has it (of the last page
+// where tok is past it), and whether it is one.  Apart, and always a load: a
+// branch around it would make a loop wait for every load it has under way.
+__device__ __forceinline__ int page_of(const AttnParams& a, const int32_t* tab, int tok, int npages) {
+    return tab[min((unsigned)tok >> a.shift, (unsigned)npages - 1)];
+}
+
+__device__ __forceinline__ bool has_page(const AttnParams& a, int id, int tok, int npages) {
+    return (((unsigned)tok >> a.shift) < (unsigned)npages) & ((unsigned)id < (unsigned)a.pages);
+}
+
+// A page to read in any case: without a page the first one, and what is read
+// is masked.
+__device__ __forceinline__ int safe_page(const AttnParams& a, int id) { return (unsigned)id < (unsigned)a.pages ? id : 0; }
+
+// Offset of a block of 16 tokens.
+__device__ __forceinline__ long block_of(const AttnParams& a, int id, int tok, int kvh, int hd) {
+    const long blocks = ((long)safe_page(a, id) * a.kv_heads + kvh) << (a.shift - 4);
+    return (blocks + ((tok & ((1 << a.shift) - 1)) >> 4)) * (16 * hd);
+}
+
+// A row's columns and how the context of a tile of them is cut.
+struct Cut {
+    int steps, active, per;
+};
+
+__device__ __forceinline__ Cut cut_context(const AttnParams& a, int most) {
+    Cut c;
+    c.steps = (most + kStep - 1) / kStep;
+    c.active = (c.steps + a.min_steps - 1) / a.min_steps;
+    c.active = c.active < 1 ? 1 : (c.active > a.splits ? a.splits : c.active);
+    c.per = (c.steps + c.active - 1) / c.active;
+    if (c.per > 0) c.active = (c.steps + c.per - 1) / c.per;
+    return c;
+}
+
+// This lane's column of a tile at column `col` of a request.
+struct Column {
+    bool valid;
+    int row, head, limit;  // limit: tokens that it attends to
+
+    __device__ __forceinline__ Column(const AttnParams& a, long col, long cols, int start, int kvh) {
+        valid = col < cols;
+        row = start + (valid ? (int)(col / a.group) : 0);
+        head = kvh * a.group + (valid ? (int)(col % a.group) : 0);
+        limit = 0;
+        if (valid) {
+            limit = a.positions[row] + 1;
+            limit = limit < 0 ? 0 : (limit > a.max_context ? a.max_context : limit);
         }
     }
 };
@@ -426,162 +414,358 @@ struct Wave {
 // out = o / l, zeros for a row that attends to nothing
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 
-// WSPLIT: the workgroup's four waves share 16 columns and take every fourth
-// step (few columns: decode rows); otherwise each wave has its own 16 columns.
-// blockIdx.z is the part of the context.
-template <int HD, int QD, int PL, bool WSPLIT>
-__global__ __launch_bounds__(256) void paged_attn_kernel(AttnParams a) {
-    constexpr int CT = WSPLIT ? 16 : 64;
+// Few columns (decode rows): the workgroup's four waves share 16 columns and
+// take every fourth step of the part blockIdx.z of the context.  Bound by the
+// cache's bytes: codes go straight to registers, each read once, the next
+// step's under way while this one's are used.  (Row r of the key operand of
+// tile t is token 16 (r >> 2) + 4 t + (r & 3): a lane's 16 scores are those of
+// the 16 tokens whose values it holds, in one page.)
+template <int HD, int QD, int PL>
+__global__ __launch_bounds__(256) void paged_attn_rows_kernel(AttnParams a) {
+    using W = Wave<HD, QD, PL>;
+    constexpr int NS = W::NS, ND = W::ND;
     constexpr int LDO = HD + 4;
-    __shared__ __align__(16) float o_s[WSPLIT ? 4 * 16 * LDO : 1];
-    __shared__ float ml_s[WSPLIT ? 4 * 16 * 2 : 1];
+    __shared__ __align__(16) float o_s[4 * 16 * LDO];
+    __shared__ float ml_s[4 * 16 * 2];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.y, part = blockIdx.z;
     int first_tile;
-    // the last tiles of a chunk attend to the most: they start first
-    const int x = WSPLIT ? blockIdx.x : gridDim.x - 1 - blockIdx.x;
-    const int r = find_request(a, CT, x, lane, &first_tile);
+    const int r = find_request(a, 16, blockIdx.x, lane, &first_tile);
     if (r < 0) return;
     int start = a.row_start[r], end = a.row_start[r + 1];
     start = start < 0 ? 0 : start;
     end = end > a.rows ? a.rows : end;
     const long cols = (long)(end - start) * a.group;
-    const long c0 = (long)(x - first_tile) * CT;
-    if (c0 >= cols || cols < a.lo_cols || cols > a.hi_cols) return;
-    const long col = c0 + (WSPLIT ? 0 : 16 * wave) + n;
-    const bool valid = col < cols;
-    const int row = start + (valid ? (int)(col / a.group) : 0);
-    const int head = kvh * a.group + (valid ? (int)(col % a.group) : 0);
-    int limit = 0;  // tokens this column attends to
-    if (valid) {
-        limit = a.positions[row] + 1;
-        limit = limit < 0 ? 0 : (limit > a.max_context ? a.max_context : limit);
-    }
-    int most = limit;
-    int least = valid ? limit : 0x7fffffff;
+    const long c0 = (long)(blockIdx.x - first_tile) * 16;
+    if (c0 >= cols || cols > a.hi_cols) return;
+    const Column me(a, c0 + n, cols, start, kvh);
+    int most = me.limit;
+    int least = me.valid ? me.limit : 0x7fffffff;
 #pragma unroll
     for (int d = 8; d >= 1; d >>= 1) {
         most = max(most, __shfl_xor(most, d, 64));
         least = min(least, __shfl_xor(least, d, 64));
     }
-    const int steps = (most + kStep - 1) / kStep;
-    int active = (steps + a.min_steps - 1) / a.min_steps;
-    active = active < 1 ? 1 : (active > a.splits ? a.splits : active);
-    const int per = (steps + active - 1) / active;
-    if (per > 0) active = (steps + per - 1) / per;
-    if (part >= active) return;
-    if (WSPLIT ? false : c0 + 16 * wave >= cols) return;
+    const Cut cut = cut_context(a, most);
+    if (part >= cut.active) return;
 
-    Wave<HD, QD, PL> w;
+    W w;
     w.clear();
-    const long rh = (long)row * a.heads + head;
-    const int s0 = part * per, s1 = min(s0 + per, steps);
-    const int first = s0 + (WSPLIT ? wave : 0), stride = WSPLIT ? 4 : 1;
+    const int s1 = min((part + 1) * cut.per, cut.steps);
+    const int first = part * cut.per + wave;
     if (first < s1) {
         const int32_t* tab = a.table + (long)r * a.max_pages;
         const int npages = (most + (1 << a.shift) - 1) >> a.shift;
-        using W = Wave<HD, QD, PL>;
-        typename W::Codes c;
-        typename W::Pages pg = W::pages_of(a, tab, first * kStep, npages, n, g);
-        W::load_k(a, pg, first * kStep, kvh, n, g, c);
-        W::load_scales(a, pg, kvh, c);
-        W::load_v(a, pg, first * kStep, kvh, n, g, c);
-        pg = W::pages_of(a, tab, (first + stride) * kStep, npages, n, g);
-        w.load_q(a, (long)row * a.q_stride + (long)head * HD, valid, g);
+        v4i k[4][NS], v[ND];
+        float ks, vs;
+        int pk, pv;  // pages of this lane's key row and of its 16 tokens
+        auto pages = [&](int tok0) {
+            pk = page_of(a, tab, tok0 + 16 * (n >> 2), npages);
+            pv = page_of(a, tab, tok0 + 16 * g, npages);
+        };
+        auto keys = [&](int page, int tok0) {
+            const int8_t* p = a.k + block_of(a, page, tok0 + 16 * (n >> 2), kvh, HD) + 256 * g + 16 * (n & 3);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    if (HD >= 64 || 16 * g < HD) k[t][s] = ldg(p + 64 * t + 1024 * s);
+                    else k[t][s] = v4i{0, 0, 0, 0};
+                }
+            }
+        };
+        auto scales = [&](int page) {
+            const long at = (long)safe_page(a, page) * a.kv_heads + kvh;
+            ks = a.ks[at];
+            vs = a.vs[at];
+        };
+        auto values = [&](int page, int tok0) {
+            const int8_t* p = a.v + block_of(a, page, tok0 + 16 * g, kvh, HD) + 16 * n;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) v[d] = ldg(p + 256 * d);
+        };
+        v8h ph[2], pl[2];
+        auto finish = [&](float* x, float ks_, float vs_, bool ok, int tok0) {
+            const float f = w.qf * ks_, fs[4] = {f, f, f, f};
+            const float vo = ok ? vs_ : 0.0f, vv[4] = {vo, vo, vo, vo};
+            const int left = ok ? me.limit - (tok0 + 16 * g) : 0;
+            w.softmax(x, fs, vv, column_max(vo), tok0 + kStep <= least && __all(ok), [&](int i) { return i < left; }, ph, pl);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                uint32_t c[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) codes_f16((uint32_t)v[d][j], c + 2 * j);
+                w.value(d, __builtin_bit_cast(v8h, v4i{(int)c[0], (int)c[1], (int)c[2], (int)c[3]}), ph[0], pl[0]);
+                w.value(d, __builtin_bit_cast(v8h, v4i{(int)c[4], (int)c[5], (int)c[6], (int)c[7]}), ph[1], pl[1]);
+            }
+        };
+        pages(first * kStep);
+        keys(pk, first * kStep);
+        scales(pv);
+        values(pv, first * kStep);
+        int pk1 = pk, pv1 = pv;
+        pages((first + 4) * kStep);
+        w.load_q(a, (long)me.row * a.q_stride + (long)me.head * HD, me.valid, g);
         // the next step's keys are on their way from the end of this step's
         // scores on, its values from the end of this step's product, its page
         // numbers a step earlier
         int s = first;
         float x[16];
-        v8h ph[2], pl[2];
-        for (; s + stride < s1; s += stride) {
-            const int tok0 = s * kStep, tok1 = (s + stride) * kStep;
-            w.scores(c, x);
-            const float ks = c.ks, vs = c.vs;
-            const bool ok = c.ok;
-            const typename W::Pages now = pg;
-            W::load_k(a, now, tok1, kvh, n, g, c);
-            W::load_scales(a, now, kvh, c);
-            pg = W::pages_of(a, tab, tok1 + stride * kStep, npages, n, g);
-            w.softmax(x, ks, vs, ok, tok0, g, limit, tok0 + kStep <= least && __all(ok), ph, pl);
-            w.values(c, ph, pl);
-            W::load_v(a, now, tok1, kvh, n, g, c);
-        }
-        w.scores(c, x);
-        w.softmax(x, c.ks, c.vs, c.ok, s * kStep, g, limit, s * kStep + kStep <= least && __all(c.ok), ph, pl);
-        w.values(c, ph, pl);
-    }
-    float l = w.l;
-    l += shfl_xor_f(l, 16);
-    l += shfl_xor_f(l, 32);
-    const float unit = w.ref / kPeak;
-    float* part_o = a.part_o + ((long)part * a.rows * a.heads + rh) * HD;
-    float* part_ml = a.part_ml + ((long)part * a.rows * a.heads + rh) * 2;
-    if (WSPLIT) {
-        // join the four waves' parts
+        for (; s + 4 < s1; s += 4) {
 #pragma unroll
-        for (int d = 0; d < HD / 16; ++d) {
-            const v4f y = w.o[d] * unit;
-            *(v4f*)&o_s[(wave * 16 + n) * LDO + 16 * d + 4 * g] = y;
+            for (int t = 0; t < 4; ++t) w.tile(k[t], x + 4 * t);
+            const float ks0 = ks, vs0 = vs;
+            const bool ok = has_page(a, pv1, s * kStep + 16 * g, npages);
+            pk1 = pk, pv1 = pv;
+            keys(pk1, (s + 4) * kStep);
+            scales(pv1);
+            pages((s + 8) * kStep);
+            finish(x, ks0, vs0, ok, s * kStep);
+            values(pv1, (s + 4) * kStep);
         }
-        if (g == 0) {
-            ml_s[(wave * 16 + n) * 2] = w.m;
-            ml_s[(wave * 16 + n) * 2 + 1] = l;
-        }
-        __syncthreads();
-        // thread t: column t / 16, dimensions 4 (t % 16) + 64 i
-        const int cn = threadIdx.x >> 4, d0 = 4 * (threadIdx.x & 15);
-        if (c0 + cn >= cols) return;
-        float m = kNegInf;
-        for (int i = 0; i < 4; ++i) m = fmaxf(m, ml_s[(i * 16 + cn) * 2]);
-        float wt[4], sum = 0.0f;
-        for (int i = 0; i < 4; ++i) {
-            const float mi = ml_s[(i * 16 + cn) * 2];
-            wt[i] = mi == m ? 1.0f : __builtin_amdgcn_exp2f(mi - m);
-            sum += wt[i] * ml_s[(i * 16 + cn) * 2 + 1];
-        }
-        const int crow = start + (int)((c0 + cn) / a.group), chead = kvh * a.group + (int)((c0 + cn) % a.group);
-        const long crh = (long)crow * a.heads + chead;
-        const float inv = active == 1 ? inverse_sum(sum) : 1.0f;
-        for (int d = d0; d < HD; d += 64) {
-            float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int i = 0; i < 4; ++i) {
-                const v4f p = *(const v4f*)&o_s[(i * 16 + cn) * LDO + d];
-                for (int j = 0; j < 4; ++j) y[j] += wt[i] * p[j];
-            }
-            for (int j = 0; j < 4; ++j) y[j] *= inv;
-            if (active == 1) store4(a.out, a.type, (long)crow * a.out_stride + (long)chead * HD + d, a.vec, y);
-            else *(float4*)&a.part_o[((long)part * a.rows * a.heads + crh) * HD + d] = make_float4(y[0], y[1], y[2], y[3]);
-        }
-        if ((threadIdx.x & 15) == 0 && a.splits > 1) {
-            if (active > 1) {
-                float* ml = a.part_ml + ((long)part * a.rows * a.heads + crh) * 2;
-                ml[0] = m;
-                ml[1] = sum;
-            }
-            if (part == 0) a.active[crh] = active;
-        }
-        return;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) w.tile(k[t], x + 4 * t);
+        finish(x, ks, vs, has_page(a, pv1, s * kStep + 16 * g, npages), s * kStep);
     }
-    if (!valid) return;
-    if (active == 1) {
+    // join the four waves' parts
+    const float l = column_sum(w.l), unit = w.ref / kPeak;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) *(v4f*)&o_s[(wave * 16 + n) * LDO + 16 * d + 4 * g] = w.o[d] * unit;
+    if (g == 0) {
+        ml_s[(wave * 16 + n) * 2] = w.m;
+        ml_s[(wave * 16 + n) * 2 + 1] = l;
+    }
+    __syncthreads();
+    // thread t: column t / 16, dimensions 4 (t % 16) + 64 i
+    const int cn = threadIdx.x >> 4, d0 = 4 * (threadIdx.x & 15);
+    if (c0 + cn >= cols) return;
+    float m = kNegInf;
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, ml_s[(i * 16 + cn) * 2]);
+    float wt[4], sum = 0.0f;
+    for (int i = 0; i < 4; ++i) {
+        const float mi = ml_s[(i * 16 + cn) * 2];
+        wt[i] = mi == m ? 1.0f : __builtin_amdgcn_exp2f(mi - m);
+        sum += wt[i] * ml_s[(i * 16 + cn) * 2 + 1];
+    }
+    const int row = start + (int)((c0 + cn) / a.group), head = kvh * a.group + (int)((c0 + cn) % a.group);
+    const long rh = (long)row * a.heads + head, all = (long)a.rows * a.heads;
+    const float inv = cut.active == 1 ? inverse_sum(sum) : 1.0f;
+    for (int d = d0; d < HD; d += 64) {
+        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < 4; ++i) {
+            const v4f p = *(const v4f*)&o_s[(i * 16 + cn) * LDO + d];
+            for (int j = 0; j < 4; ++j) y[j] += wt[i] * p[j];
+        }
+        for (int j = 0; j < 4; ++j) y[j] *= inv;
+        if (cut.active == 1) store4(a.out, a.type, (long)row * a.out_stride + (long)head * HD + d, a.vec, y);
+        else *(float4*)&a.part_o[(part * all + rh) * HD + d] = make_float4(y[0], y[1], y[2], y[3]);
+    }
+    if ((threadIdx.x & 15) == 0 && a.splits > 1) {
+        if (cut.active > 1) {
+            a.part_ml[(part * all + rh) * 2] = m;
+            a.part_ml[(part * all + rh) * 2 + 1] = sum;
+        }
+        if (part == 0) a.active[rh] = cut.active;
+    }
+}
+
+// Many columns of one request (chunks of prompts): eight waves of 16 columns
+// each go through the part's steps together.  Bound by vector instructions
+// (about 15 for each score, exp2 among them), so what the waves can share is
+// done once: a step's codes are staged in LDS, keys as stored, values as fp16,
+// in the order of the operands (whole-line reads without bank conflicts), and
+// few enough registers stay that four waves share a SIMD (head_dim up to 128).
+// Row r of the key operand of tile t is token 16 t + r here: a lane's scores
+// are tokens 16 t + 4 g + i, and the values' tokens are written in that order.
+// Two buffers, one barrier a step.
+constexpr int kChunkWaves = 4;
+constexpr int kChunkCols = 16 * kChunkWaves;
+
+template <int HD, int QD, int PL>
+__global__ __launch_bounds__(64 * kChunkWaves, HD <= 128 ? 3 : 1) void paged_attn_chunk_kernel(AttnParams a) {
+    using W = Wave<HD, QD, PL>;
+    constexpr int NS = W::NS, ND = W::ND, THREADS = 64 * kChunkWaves;
+    constexpr int KU = 4 * HD;                           // 16-byte units of a step's keys, and of its values
+    constexpr int PER = (2 * KU + THREADS - 1) / THREADS;  // units of a thread
+    struct Scales {
+        float k[4], v[4];
+        int ok;
+        float vmax;
+    };
+    __shared__ v4i k_s[2][KU];
+    __shared__ v4i v_s[2][2 * KU];
+    __shared__ Scales sc_s[2];
+    __shared__ int most_s[kChunkWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.y, part = blockIdx.z;
+    int first_tile;
+    // the last tiles of a chunk attend to the most: they start first
+    const int x0 = gridDim.x - 1 - blockIdx.x;
+    const int r = find_request(a, kChunkCols, x0, lane, &first_tile);
+    if (r < 0) return;
+    int start = a.row_start[r], end = a.row_start[r + 1];
+    start = start < 0 ? 0 : start;
+    end = end > a.rows ? a.rows : end;
+    const long cols = (long)(end - start) * a.group;
+    const long c0 = (long)(x0 - first_tile) * kChunkCols;
+    if (c0 >= cols || cols <= a.hi_cols) return;
+    const Column me(a, c0 + 16 * wave + n, cols, start, kvh);
+    int mine = me.limit;
+    int least = me.valid ? me.limit : 0x7fffffff;
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) {
+        mine = max(mine, __shfl_xor(mine, d, 64));
+        least = min(least, __shfl_xor(least, d, 64));
+    }
+    if (lane == 0) most_s[wave] = mine;
+    __syncthreads();
+    int most = 0;
+#pragma unroll
+    for (int i = 0; i < kChunkWaves; ++i) most = max(most, most_s[i]);
+    const Cut cut = cut_context(a, most);
+    if (part >= cut.active) return;
+
+    W w;
+    w.clear();
+    const int s0 = part * cut.per, s1 = min(s0 + cut.per, cut.steps);
+    if (s0 < s1) {
+        const int32_t* tab = a.table + (long)r * a.max_pages;
+        const int npages = (most + (1 << a.shift) - 1) >> a.shift;
+        // unit u of a step: keys (u < KU) or values, block (u % KU) / HD, 16 bytes
+        // u % HD of it
+        int page[PER], page_sc;
+        v4i code[PER];
+        float sk, sv;
+        auto pages = [&](int tok0) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) page[i] = page_of(a, tab, tok0 + 16 * (((threadIdx.x + THREADS * i) % KU) / HD), npages);
+            page_sc = page_of(a, tab, tok0 + 16 * (lane & 3), npages);
+        };
+        auto fetch = [&](int tok0) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int u = threadIdx.x + THREADS * i;
+                if (2 * KU % THREADS == 0 || u < 2 * KU) {
+                    const long at = block_of(a, page[i], tok0 + 16 * ((u % KU) / HD), kvh, HD) + 16 * (u % HD);
+                    code[i] = ldg((u < KU ? a.k : a.v) + at);
+                }
+            }
+            const long at = (long)safe_page(a, page_sc) * a.kv_heads + kvh;
+            sk = a.ks[at];
+            sv = a.vs[at];
+        };
+        auto stage = [&](int b, int sc_page, int tok0) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int u = threadIdx.x + THREADS * i;
+                if (u < KU) {
+                    k_s[b][u] = code[i];
+                } else if (2 * KU % THREADS == 0 || u < 2 * KU) {
+                    // dimension d of block t: its tokens 4 g .. are lane (d % 16, g)'s
+                    const int t = (u - KU) / HD, d = (u - KU) % HD;
+                    uint2* to = (uint2*)&v_s[b][((t >> 1) * ND + (d >> 4)) * 64 + (d & 15)] + (t & 1);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t c[2];
+                        codes_f16((uint32_t)code[i][j], c);
+                        to[j * 32] = make_uint2(c[0], c[1]);
+                    }
+                }
+            }
+            if (wave == kChunkWaves - 1) {
+                const bool ok = has_page(a, sc_page, tok0 + 16 * (lane & 3), npages);
+                const float v = ok ? sv : 0.0f;
+                float vm = fmaxf(v, __shfl_xor(v, 1, 64));
+                vm = fmaxf(vm, __shfl_xor(vm, 2, 64));
+                const unsigned long long all = __ballot(ok);
+                if (lane < 4) {
+                    sc_s[b].k[lane] = sk;
+                    sc_s[b].v[lane] = v;
+                }
+                if (lane == 0) {
+                    sc_s[b].ok = (int)(all & 15);
+                    sc_s[b].vmax = vm;
+                }
+            }
+        };
+        pages(s0 * kStep);
+        fetch(s0 * kStep);
+        int sc_page = page_sc;
+        pages((s0 + 1) * kStep);
+        w.load_q(a, (long)me.row * a.q_stride + (long)me.head * HD, me.valid, g);
+        stage(0, sc_page, s0 * kStep);
+        __syncthreads();
+        const int my_steps = (mine + kStep - 1) / kStep;
+        for (int s = s0; s < s1; ++s) {
+            const int b = (s - s0) & 1;
+            const bool more = s + 1 < s1;
+            if (more) {
+                fetch((s + 1) * kStep);
+                sc_page = page_sc;
+                pages((s + 2) * kStep);
+            }
+            if (s < my_steps) {
+                float x[16];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    v4i k[NS];
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) {
+                        if (HD >= 64 || 16 * g < HD) k[i] = k_s[b][t * HD + (g + 4 * i) * 16 + n];
+                        else k[i] = v4i{0, 0, 0, 0};
+                    }
+                    w.tile(k, x + 4 * t);
+                }
+                const Scales& sc = sc_s[b];
+                const int ok = sc.ok;
+                const float f[4] = {w.qf * sc.k[0], w.qf * sc.k[1], w.qf * sc.k[2], w.qf * sc.k[3]};
+                const float vs[4] = {sc.v[0], sc.v[1], sc.v[2], sc.v[3]};
+                const int left = me.limit - (s * kStep + 4 * g);
+                v8h ph[2], pl[2];
+                w.softmax(x, f, vs, sc.vmax, s * kStep + kStep <= least && ok == 15,
+                          [&](int i) { return 16 * (i >> 2) + (i & 3) < left && (ok >> (i >> 2) & 1); }, ph, pl);
+                // operand reads kAhead ahead of the products that take them (left
+                // alone, the compiler waits for each)
+                constexpr int kAhead = 4;
+                v4i vb[kAhead];
+                auto operand = [&](int i) { return v_s[b][((i & 1) * ND + (i >> 1)) * 64 + lane]; };
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) vb[i] = operand(i);
+#pragma unroll
+                for (int i = 0; i < 2 * ND; ++i) {
+                    const v4i v = vb[i % kAhead];
+                    __builtin_amdgcn_sched_barrier(0);
+                    w.value(i >> 1, __builtin_bit_cast(v8h, v), ph[i & 1], pl[i & 1]);
+                    if (i + kAhead < 2 * ND) vb[i % kAhead] = operand(i + kAhead);
+                }
+            }
+            if (more) stage(b ^ 1, sc_page, (s + 1) * kStep);
+            __syncthreads();
+        }
+    }
+    const float l = column_sum(w.l), unit = w.ref / kPeak;
+    if (!me.valid) return;
+    const long rh = (long)me.row * a.heads + me.head;
+    if (cut.active == 1) {
         const float inv = inverse_sum(l) * unit;
 #pragma unroll
-        for (int d = 0; d < HD / 16; ++d) {
+        for (int d = 0; d < ND; ++d) {
             float y[4];
             for (int j = 0; j < 4; ++j) y[j] = w.o[d][j] * inv;
-            store4(a.out, a.type, (long)row * a.out_stride + (long)head * HD + 16 * d + 4 * g, a.vec, y);
+            store4(a.out, a.type, (long)me.row * a.out_stride + (long)me.head * HD + 16 * d + 4 * g, a.vec, y);
         }
     } else {
+        const long at = (long)part * a.rows * a.heads + rh;
 #pragma unroll
-        for (int d = 0; d < HD / 16; ++d) *(v4f*)&part_o[16 * d + 4 * g] = w.o[d] * unit;
+        for (int d = 0; d < ND; ++d) *(v4f*)&a.part_o[at * HD + 16 * d + 4 * g] = w.o[d] * unit;
         if (g == 0) {
-            part_ml[0] = w.m;
-            part_ml[1] = l;
+            a.part_ml[at * 2] = w.m;
+            a.part_ml[at * 2 + 1] = l;
         }
     }
-    if (a.splits > 1 && part == 0 && g == 0) a.active[rh] = active;
+    if (a.splits > 1 && part == 0 && g == 0) a.active[rh] = cut.active;
 }
 
 // Joins the parts of rows whose context was cut: one wave per (row, head).
@@ -662,23 +846,19 @@ size_t paged_attn_workspace(int rows, int heads, int kv_heads, int hd, int reque
 
 template <int HD, int QD, int PL>
 static hipError_t launch_typed(AttnParams& a, hipStream_t s) {
-    const int group = a.group;
-    const long cols = (long)a.rows * group;
-    const int kAll = 0x7fffffff;
-    // requests of at most 16 columns (decode rows) take the wave-split kernel;
-    // where every request may be one, it takes all of them
+    const long cols = (long)a.rows * a.group;
+    // requests of at most 16 columns (decode rows) take the rows kernel; where
+    // every request may be one, it takes all of them
     const bool few = cols <= 16l * a.requests;
-    a.lo_cols = 1;
-    a.hi_cols = few ? kAll : 16;
-    hipLaunchKernelGGL((paged_attn_kernel<HD, QD, PL, true>),
+    a.hi_cols = few ? 0x7fffffff : 16;
+    hipLaunchKernelGGL((paged_attn_rows_kernel<HD, QD, PL>),
                        dim3((unsigned)(cols / 16 + a.requests), (unsigned)a.kv_heads, (unsigned)a.splits), dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (!few) {
-        a.lo_cols = 17;
-        a.hi_cols = kAll;
-        hipLaunchKernelGGL((paged_attn_kernel<HD, QD, PL, false>),
-                           dim3((unsigned)(cols / 64 + a.requests), (unsigned)a.kv_heads, (unsigned)a.splits), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((paged_attn_chunk_kernel<HD, QD, PL>),
+                           dim3((unsigned)(cols / kChunkCols + a.requests), (unsigned)a.kv_heads, (unsigned)a.splits),
+                           dim3(64 * kChunkWaves), 0, s, a);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
