@@ -36,6 +36,7 @@ constexpr unsigned long long kDefMask = (1ull << 48) - 1;
 struct SegMax {
     float value;  // -inf: no token of the segment can be drawn
     int index;
+    int listed;   // tokens of its list
 };
 
 __device__ __forceinline__ float usable(float x) {  // NaN: never drawn; +inf: the largest finite value
@@ -129,14 +130,57 @@ struct SampleParams {
     int32_t* ids;
     SegMax* seg_max;            // [row][seg]
     unsigned long long* hist;   // [row][seg][kBuckets]: count << 48 | deficits
+    uint16_t* first;            // [row][seg][kBuckets]: where a bucket's tokens start in the list
+    uint16_t* list;             // [row][seg][kSeg]: tokens (within the segment) by bucket
 };
 
-// One workgroup per (segment, row): its largest value and its histogram
-// relative to it.  A bucket's mass is kept as count and sum of 1 - exp(distance
-// to the bucket's upper edge), one 64-bit LDS atomic a token, which is exact
-// in any order and needs the row's maximum only when segments are joined.
+struct Filters {
+    float temperature, top_p, min_p;
+    int top_k;
+
+    __device__ __forceinline__ Filters(const SampleParams& a, long row) {
+        temperature = a.temperature ? a.temperature[row] : 1.0f;
+        top_k = a.top_k ? a.top_k[row] : 0;
+        top_p = a.top_p ? a.top_p[row] : 1.0f;
+        min_p = a.min_p ? a.min_p[row] : 0.0f;
+    }
+    __device__ __forceinline__ bool any(int vocab) const {
+        return (top_k > 0 && top_k < vocab) || top_p < 1.0f || min_p > 0.0f;
+    }
+};
+
+// Inclusive sums over the workgroup in thread order, and their total.
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, T* wave_sum, T* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const T o = __shfl_up(v, d, 64);
+        if (lane >= d) v += o;
+    }
+    __syncthreads();
+    if (lane == 63) wave_sum[wave] = v;
+    __syncthreads();
+    T before = 0, all = 0;
+    for (int w = 0; w < kThreads / 64; ++w) {
+        const T x = wave_sum[w];
+        if (w < wave) before += x;
+        all += x;
+    }
+    *total = all;
+    return v + before;
+}
+
+// One workgroup per (segment, row): its largest value, its histogram relative
+// to it, and (where a filter may ask) its tokens listed by bucket.  A bucket's
+// mass is kept as count and sum of 1 - exp(distance to the bucket's upper
+// edge), one 64-bit LDS atomic a token, which is exact in any order and needs
+// the row's maximum only when segments are joined; the atomic's old count is
+// the token's place in its bucket's list.
 __global__ __launch_bounds__(kThreads) void sample_segments_kernel(SampleParams a) {
     __shared__ unsigned long long hist[kBuckets];
+    __shared__ uint16_t first[kBuckets];
+    __shared__ __align__(16) uint16_t list[kSeg];
     __shared__ float sv[kThreads / 64];
     __shared__ int si[kThreads / 64];
     const int tid = threadIdx.x, seg = blockIdx.y;
@@ -149,6 +193,7 @@ __global__ __launch_bounds__(kThreads) void sample_segments_kernel(SampleParams 
         l[4 * j] = usable(f.x), l[4 * j + 1] = usable(f.y), l[4 * j + 2] = usable(f.z), l[4 * j + 3] = usable(f.w);
     }
     hist[tid] = 0;
+    const Filters fl(a, row);
     float best = -__builtin_inff();
     int at = 0x7fffffff;
 #pragma unroll
@@ -158,26 +203,47 @@ __global__ __launch_bounds__(kThreads) void sample_segments_kernel(SampleParams 
     }
     block_best(best, at, sv, si);
     const long slot = row * a.segs + seg;
-    if (tid == 0) a.seg_max[slot] = SegMax{best, at};
-    const float temp = a.temperature ? a.temperature[row] : 1.0f;
-    if (!(temp > 0.0f)) return;  // greedy: the maximum is all
-    if (best > -__builtin_inff()) {
-        const double inv_t = 1.0 / (double)temp;
-        const Place top = place(best, inv_t);
-        const bool far = fabs(top.z) >= kFar;
+    if (!(fl.temperature > 0.0f) || best == -__builtin_inff()) {  // greedy, or nothing to draw: the maximum is all
+        if (tid == 0) a.seg_max[slot] = SegMax{best, at, 0};
+        return;
+    }
+    const double inv_t = 1.0 / (double)fl.temperature;
+    const Place top = place(best, inv_t);
+    const bool far = fabs(top.z) >= kFar;
+    int place_of[8];  // bucket << 16 | place in it
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (l[i] == -__builtin_inff()) continue;
-            const Place p = place(l[i], inv_t);
-            const int d = bucket_of(p, top);
-            if (d >= kBuckets) continue;
-            double r = far ? 0.0 : (p.z - (p.b + 1.0) / kPerNat) + p.lo;
-            r = fmin(fmax(r, -1.0 / kPerNat), 0.0);
-            atomicAdd(&hist[d], (1ull << 48) | (unsigned long long)(deficit(r) * kDefUnit + 0.5));
-        }
+    for (int i = 0; i < 8; ++i) {
+        place_of[i] = -1;
+        if (l[i] == -__builtin_inff()) continue;
+        const Place p = place(l[i], inv_t);
+        const int d = bucket_of(p, top);
+        if (d >= kBuckets) continue;
+        double r = far ? 0.0 : (p.z - (p.b + 1.0) / kPerNat) + p.lo;
+        r = fmin(fmax(r, -1.0 / kPerNat), 0.0);
+        const unsigned long long old = atomicAdd(&hist[d], (1ull << 48) | (unsigned long long)(deficit(r) * kDefUnit + 0.5));
+        place_of[i] = d << 16 | (int)(old >> 48);
     }
     __syncthreads();
-    a.hist[slot * kBuckets + tid] = hist[tid];
+    const unsigned long long h = hist[tid];
+    a.hist[slot * kBuckets + tid] = h;
+    int listed = 0;
+    if (fl.any(a.vocab)) {
+        const int n = (int)(h >> 48);
+        const int end = block_scan(n, si, &listed);
+        first[tid] = (uint16_t)(end - n);
+        a.first[slot * kBuckets + tid] = (uint16_t)(end - n);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (place_of[i] >= 0) {
+                list[first[place_of[i] >> 16] + (place_of[i] & 0xffff)] =
+                    (uint16_t)(4 * tid + (i >> 2) * 4 * kThreads + (i & 3));
+            }
+        }
+        __syncthreads();
+        if (8 * tid < listed) ((uint4*)(a.list + slot * kSeg))[tid] = ((const uint4*)list)[tid];
+    }
+    if (tid == 0) a.seg_max[slot] = SegMax{best, at, listed};
 }
 
 // What a row keeps: buckets up to `bucket`, and of those the tokens ranked at
@@ -197,64 +263,28 @@ struct PickShared {
     int list_idx[kList];
     unsigned long long part[kMaxSegs];  // kept mass of the cut's bucket by segment
     double seg_mass[kMaxSegs];
+    int shift[kMaxSegs];  // a segment's buckets start so many below the row's (kBuckets: none)
     double wave_d[kThreads / 64];
     long long wave_i[kThreads / 64];
     float sv[kThreads / 64];
     int si[kThreads / 64];
     int n, found_i, found_j;
     uint32_t found_key, lo_key, hi_key;
+    unsigned long long lo_ord, hi_ord, list_ord[64];
     double found_mass;
 };
 
-// Inclusive sums over the workgroup in thread order.
-__device__ __forceinline__ double scan_d(double v, double* wave_sum, double* total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const double o = __shfl_up(v, d, 64);
-        if (lane >= d) v += o;
-    }
-    __syncthreads();
-    if (lane == 63) wave_sum[wave] = v;
-    __syncthreads();
-    double before = 0, all = 0;
-    for (int w = 0; w < kThreads / 64; ++w) {
-        const double x = wave_sum[w];
-        if (w < wave) before += x;
-        all += x;
-    }
-    *total = all;
-    return v + before;
-}
-
-__device__ __forceinline__ long long scan_i(long long v, long long* wave_sum, long long* total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const long long o = __shfl_up(v, d, 64);
-        if (lane >= d) v += o;
-    }
-    __syncthreads();
-    if (lane == 63) wave_sum[wave] = v;
-    __syncthreads();
-    long long before = 0, all = 0;
-    for (int w = 0; w < kThreads / 64; ++w) {
-        const long long x = wave_sum[w];
-        if (w < wave) before += x;
-        all += x;
-    }
-    *total = all;
-    return v + before;
-}
-
 struct Row {
     const float* x;
-    int vocab;
+    int vocab, segs;
     bool vec;
     double inv_t;
     float max;
     Place top;
-    bool far;
+    const SegMax* seg_max;
+    const unsigned long long* hist;
+    const uint16_t* first;
+    const uint16_t* list;
 
     __device__ __forceinline__ double weight(float l) const {
         return exp(((double)l - (double)max) * inv_t);
@@ -264,33 +294,21 @@ struct Row {
     }
     __device__ __forceinline__ int bucket(float l) const { return bucket_of(place(l, inv_t), top); }
 
-    // f(value, index) for the row's tokens in buckets b0..b1 that the cut
-    // keeps; the values are read eight vectors ahead
+    // f(value, key, index) for the row's tokens in buckets b0..b1 that the cut
+    // keeps, from the segments' lists: a wave a segment
     template <typename F>
-    __device__ __forceinline__ void each(int b0, int b1, const Cut& cut, F f) const {
-        // bounds of the buckets' values, a little wide: most tokens are out
-        // with two comparisons
-        const double z0 = (top.b - b1) / kPerNat / inv_t, z1 = (top.b - b0 + 1.0) / kPerNat / inv_t;
-        // (an infinite temperature leaves 0 / 0 for the lowest)
-        const float lo = far ? max : z0 == z0 ? (float)(z0 - fabs(z0) * 1e-6) : -__builtin_inff();
-        const float hi = far ? max : z1 == z1 ? (float)(z1 + fabs(z1) * 1e-6) : __builtin_inff();
-        for (int base = 0; base < vocab; base += 32 * kThreads) {
-            float4 v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = load4(x, vocab, base + 4 * (j * kThreads + (int)threadIdx.x), vec);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float e[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float l = usable(e[i]);
-                    if (!(l >= lo && l <= hi)) continue;
-                    const int d = bucket(l);
-                    if (d < b0 || d > b1 || d >= kBuckets) continue;
-                    const int idx = base + 4 * (j * kThreads + (int)threadIdx.x) + i;
-                    const uint32_t k = key_of(l);
-                    if (k > cut.key || (k == cut.key && idx <= cut.index)) f(l, k, idx);
-                }
+    __device__ __forceinline__ void each(const PickShared& s, int b0, int b1, const Cut& cut, F f) const {
+        for (int i = threadIdx.x >> 6; i < segs; i += kThreads / 64) {
+            const int shift = s.shift[i];
+            const int d0 = b0 > shift ? b0 - shift : 0, d1 = b1 - shift;
+            if (d1 < 0 || shift >= kBuckets) continue;
+            const int from = first[(long)i * kBuckets + d0];
+            const int to = d1 + 1 < kBuckets ? first[(long)i * kBuckets + d1 + 1] : seg_max[i].listed;
+            for (int j = from + (threadIdx.x & 63); j < to; j += 64) {
+                const int idx = i * kSeg + list[(long)i * kSeg + j];
+                const float l = usable(x[idx]);
+                const uint32_t k = key_of(l);
+                if (k > cut.key || (k == cut.key && idx <= cut.index)) f(l, k, idx);
             }
         }
     }
@@ -317,7 +335,7 @@ __device__ double resolve(const Row& row, PickShared& s, int b0, int b1, long lo
         s.list_idx[tid] = 0;
         __syncthreads();
         uint32_t lo = 0xffffffffu, hi = 0;
-        row.each(b0, b1, *cut, [&](float, uint32_t k, int) {
+        row.each(s, b0, b1, *cut, [&](float, uint32_t k, int) {
             if (k >= k0 && k <= k1) lo = min(lo, k), hi = max(hi, k);
         });
         if (lo <= hi) atomicMin(&s.lo_key, lo), atomicMax(&s.hi_key, hi);
@@ -329,7 +347,7 @@ __device__ double resolve(const Row& row, PickShared& s, int b0, int b1, long lo
         }
         const int bits = 32 - __builtin_clz(hi - lo);
         const int shift = bits > 10 ? bits - 10 : 0;
-        row.each(b0, b1, *cut, [&](float l, uint32_t k, int) {
+        row.each(s, b0, b1, *cut, [&](float l, uint32_t k, int) {
             if (k < k0 || k > k1) return;
             const int at = (int)((hi - k) >> shift);
             atomicAdd(&s.list_idx[at], 1);
@@ -340,8 +358,8 @@ __device__ double resolve(const Row& row, PickShared& s, int b0, int b1, long lo
         const double w = (double)s.list_w[tid] * 0x1p-40;
         long long tc;
         double tw;
-        const long long ci = scan_i(c, s.wave_i, &tc);
-        const double wi = scan_d(w, s.wave_d, &tw) + above;
+        const long long ci = block_scan<long long>(c, s.wave_i, &tc);
+        const double wi = block_scan<double>(w, s.wave_d, &tw) + above;
         if (tid == 0) s.found_j = kThreads;
         __syncthreads();
         const bool crossed = c > 0 && (count ? ci >= left : wi >= target);
@@ -389,7 +407,7 @@ __device__ double resolve(const Row& row, PickShared& s, int b0, int b1, long lo
             int c = 0;
             for (int i = 0; i < 4; ++i) c += usable(e[i]) == l && base + 4 * tid + i <= last;
             long long all;
-            const long long upto = scan_i(c, s.wave_i, &all) + seen;
+            const long long upto = block_scan<long long>(c, s.wave_i, &all) + seen;
             if (upto >= left && upto - c < left) {
                 long long have = upto - c;
                 for (int i = 0; i < 4; ++i) {
@@ -405,28 +423,84 @@ __device__ double resolve(const Row& row, PickShared& s, int b0, int b1, long lo
     } else {
         if (tid == 0) s.n = 0;
         __syncthreads();
-        row.each(b0, b1, *cut, [&](float l, uint32_t k, int idx) {
+        row.each(s, b0, b1, *cut, [&](float l, uint32_t k, int idx) {
             if (k < k0 || k > k1) return;
             const int at = atomicAdd(&s.n, 1);
             if (at < kList) s.list_key[at] = k, s.list_idx[at] = idx, s.list_w[at] = row.fixed(l);
         });
         __syncthreads();
         const int m = s.n < kList ? s.n : kList;
-        if (tid == 0) s.found_j = -1;
+        // a token a thread, its place in the ranking as one number (value, then
+        // index); narrowed by histograms of 1024 parts until a wave's worth is
+        // left to be ranked one against the other
+        const uint32_t key = s.list_key[tid];
+        const int idx = s.list_idx[tid];
+        const unsigned long long w = s.list_w[tid];
+        const unsigned long long ord = (unsigned long long)~key << 32 | (uint32_t)idx;
+        bool open = tid < m;
+        int now = m;
+        unsigned long long done = 0;  // mass of tokens that rank before the open ones
+        while (now > 64) {
+            __syncthreads();
+            if (tid == 0) s.lo_ord = ~0ull, s.hi_ord = 0;
+            s.list_w[tid] = 0;
+            s.list_idx[tid] = 0;
+            __syncthreads();
+            if (open) atomicMin(&s.lo_ord, ord), atomicMax(&s.hi_ord, ord);
+            __syncthreads();
+            const unsigned long long lo = s.lo_ord;
+            const int bits = 64 - __builtin_clzll(s.hi_ord - lo);  // (over 64 tokens: never equal)
+            const int shift = bits > 10 ? bits - 10 : 0;
+            const int at = (int)((ord - lo) >> shift);
+            if (open) {
+                atomicAdd(&s.list_idx[at], 1);
+                atomicAdd(&s.list_w[at], w);
+            }
+            __syncthreads();
+            const int c = s.list_idx[tid];
+            const unsigned long long cw = s.list_w[tid];
+            long long tc, tw;
+            const long long ci = block_scan<long long>(c, s.wave_i, &tc);
+            const long long wi = block_scan<long long>((long long)cw, s.wave_i, &tw) + (long long)done;
+            if (tid == 0) s.found_j = kThreads, s.found_i = 0;
+            __syncthreads();
+            if (c > 0) {
+                if (count ? ci >= left : above + (double)wi * (1.0 / kMassUnit) >= target) atomicMin(&s.found_j, tid);
+                atomicMax(&s.found_i, tid);  // (mass a rounding short of the target: the last)
+            }
+            __syncthreads();
+            const int b = s.found_j < kThreads ? s.found_j : s.found_i;
+            __syncthreads();
+            if (tid == b) {
+                s.n = c;
+                s.lo_ord = (unsigned long long)(wi - (long long)cw);
+                s.wave_i[0] = ci - c;
+            }
+            __syncthreads();
+            now = s.n;
+            done = s.lo_ord;
+            left -= s.wave_i[0];
+            open = open && at == b;
+        }
         __syncthreads();
-        uint32_t key = 0;
-        int idx = 0, rank = 0;
-        unsigned long long w = 0, mass = 0;
-        if (tid < m) {
-            key = s.list_key[tid], idx = s.list_idx[tid], w = s.list_w[tid];
-            for (int j = 0; j < m; ++j) {
-                const uint32_t kj = s.list_key[j];
-                const bool b = kj > key || (kj == key && s.list_idx[j] < idx);
+        if (tid == 0) s.n = 0, s.found_j = -1;
+        __syncthreads();
+        if (open) {
+            const int at = atomicAdd(&s.n, 1);
+            s.list_ord[at] = ord;
+            s.list_w[at] = w;
+        }
+        __syncthreads();
+        if (open) {
+            int rank = 0;
+            unsigned long long mass = done;
+            for (int j = 0; j < now; ++j) {
+                const bool b = s.list_ord[j] < ord;
                 rank += b;
                 mass += b ? s.list_w[j] : 0;
             }
             const double b = above + (double)mass * (1.0 / kMassUnit), e = above + (double)(mass + w) * (1.0 / kMassUnit);
-            const bool here = count ? rank + 1 == left : (b < target || rank == 0) && (e >= target || rank + 1 == m);
+            const bool here = count ? rank + 1 == left : (b < target || rank == 0) && (e >= target || rank + 1 == now);
             if (here) {
                 s.found_key = key;
                 s.found_i = idx;
@@ -446,7 +520,7 @@ __device__ double resolve(const Row& row, PickShared& s, int b0, int b1, long lo
         }
     }
     if (narrowed) {
-        row.each(b0, b1, *cut, [&](float l, uint32_t, int idx) { atomicAdd(&s.part[idx / kSeg], row.fixed(l)); });
+        row.each(s, b0, b1, *cut, [&](float l, uint32_t, int idx) { atomicAdd(&s.part[idx / kSeg], row.fixed(l)); });
     }
     cut->bucket = b1;
     __syncthreads();
@@ -472,48 +546,56 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const long r = blockIdx.x;
     const SegMax* sm = a.seg_max + r * a.segs;
+    const Filters fl(a, r);
     float best = -__builtin_inff();
     int at = 0x7fffffff;
     for (int i = tid; i < a.segs; i += kThreads) {
-        if (Better::before(sm[i].value, sm[i].index, best, at)) best = sm[i].value, at = sm[i].index;
+        const SegMax m = sm[i];
+        if (Better::before(m.value, m.index, best, at)) best = m.value, at = m.index;
     }
     block_best(best, at, s.sv, s.si);
-    const float temp = a.temperature ? a.temperature[r] : 1.0f;
     Row row;
     row.x = a.logits + r * a.stride;
     row.vocab = a.vocab;
+    row.segs = a.segs;
     row.vec = a.vec;
-    if (!(temp > 0.0f) || best == -__builtin_inff()) {
+    if (!(fl.temperature > 0.0f) || best == -__builtin_inff()) {
         // greedy as loom_amd_greedy_sample: 0 when the first logit is NaN
-        if (tid == 0) a.ids[r] = best == -__builtin_inff() || (!(temp > 0.0f) && row.x[0] != row.x[0]) ? 0 : at;
+        if (tid == 0) a.ids[r] = best == -__builtin_inff() || (!(fl.temperature > 0.0f) && row.x[0] != row.x[0]) ? 0 : at;
         return;
     }
-    row.inv_t = 1.0 / (double)temp;
+    row.inv_t = 1.0 / (double)fl.temperature;
     row.max = best;
     row.top = place(best, row.inv_t);
-    row.far = fabs(row.top.z) >= kFar;
+    row.seg_max = sm;
+    row.hist = a.hist + r * a.segs * kBuckets;
+    row.first = a.first + r * a.segs * kBuckets;
+    row.list = a.list + r * a.segs * kSeg;
+    const bool far = fabs(row.top.z) >= kFar;
 
     // the segments' histograms on the row's grid
+    for (int i = tid; i < a.segs; i += kThreads) {
+        const float v = sm[i].value;
+        s.shift[i] = v == -__builtin_inff() ? kBuckets : bucket_of(place(v, row.inv_t), row.top);
+    }
+    __syncthreads();
     unsigned long long def = 0;
     int cnt = 0;
+#pragma unroll 8
     for (int i = 0; i < a.segs; ++i) {
-        const float v = sm[i].value;
-        if (v == -__builtin_inff()) continue;
-        const int shift = bucket_of(place(v, row.inv_t), row.top);
-        if (tid >= shift) {
-            const unsigned long long h = a.hist[(r * a.segs + i) * kBuckets + tid - shift];
-            cnt += (int)(h >> 48);
-            def += h & kDefMask;
-        }
+        const int d = tid - s.shift[i];
+        const unsigned long long h = d >= 0 ? row.hist[(long)i * kBuckets + d] : 0;
+        cnt += (int)(h >> 48);
+        def += h & kDefMask;
     }
-    const double edge = row.far ? (tid == 0 ? 0.0 : -1e30) : ((row.top.b - tid + 1.0) / kPerNat - row.top.z) - row.top.lo;
+    const double edge = far ? (tid == 0 ? 0.0 : -1e30) : ((row.top.b - tid + 1.0) / kPerNat - row.top.z) - row.top.lo;
     const double factor = exp(edge);
     s.factor[tid] = factor;
     long long tokens;
     double whole;
-    const long long cum_n = scan_i(cnt, s.wave_i, &tokens);
+    const long long cum_n = block_scan<long long>(cnt, s.wave_i, &tokens);
     const double own = ((double)cnt - (double)def * (1.0 / kDefUnit)) * factor;
-    const double cum_w = scan_d(own, s.wave_d, &whole);
+    const double cum_w = block_scan<double>(own, s.wave_d, &whole);
     s.count[tid] = (int)cum_n;
     s.mass[tid] = cum_w;
     __syncthreads();
@@ -524,7 +606,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams a) {
     auto count_before = [&](int b) { return b > 0 ? s.count[b - 1] : 0; };
     auto mass_before = [&](int b) { return b > 0 ? s.mass[b - 1] : 0.0; };
 
-    const long long k = a.top_k ? a.top_k[r] : 0;
+    const long long k = fl.top_k;
     if (k > 0 && k < tokens) {
         const int b = first_bucket(s, [&](int i) { return s.count[i] >= k; });
         const long long nb = s.count[b] - count_before(b), take = k - count_before(b);
@@ -537,7 +619,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams a) {
             full = b;
         }
     }
-    const double p = a.top_p ? (double)a.top_p[r] : 1.0;
+    const double p = (double)fl.top_p;
     if (p < 1.0) {
         const double target = p > 0.0 ? p * kept - kSame * kept : 0.0;
         int b = first_bucket(s, [&](int i) { return s.count[i] > 0 && s.mass[i] >= target; });
@@ -546,7 +628,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams a) {
         kept = resolve(row, s, b, b, nb, 0, target, mass_before(b), &cut);
         full = b;
     }
-    double mp = a.min_p ? (double)a.min_p[r] : 0.0;
+    double mp = (double)fl.min_p;
     if (mp > 1.0) mp = 1.0;
     if (mp > 0.0) {
         // buckets that are neither whole above min_p nor whole below it
@@ -556,13 +638,13 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams a) {
         if (b1 > cut.bucket) b1 = cut.bucket;
         if (b0 <= b1) {
             int mine = 0, of = 0;
-            row.each(b0, b1, cut, [&](float l, uint32_t, int) {
+            row.each(s, b0, b1, cut, [&](float l, uint32_t, int) {
                 ++of;
                 mine += row.weight(l) >= mp;
             });
             long long got, all;
-            (void)scan_i(mine, s.wave_i, &got);
-            (void)scan_i(of, s.wave_i, &all);
+            (void)block_scan<long long>(mine, s.wave_i, &got);
+            (void)block_scan<long long>(of, s.wave_i, &all);
             if (got == 0 && b0 > 0) {
                 cut.bucket = b0 - 1;
                 full = b0;
@@ -582,14 +664,14 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams a) {
 
     // the segment where the kept mass passes u of the whole
     for (int i = wave; i < a.segs; i += kThreads / 64) {
-        const float v = sm[i].value;
+        const int shift = s.shift[i];
         double m = 0.0;
-        if (v > -__builtin_inff()) {
-            const int shift = bucket_of(place(v, row.inv_t), row.top);
-            for (int d = lane + shift; d < full && d < kBuckets; d += 64) {
-                const unsigned long long h = a.hist[(r * a.segs + i) * kBuckets + d - shift];
-                m += ((double)(h >> 48) - (double)(h & kDefMask) * (1.0 / kDefUnit)) * s.factor[d];
-            }
+#pragma unroll 8
+        for (int j = 0; j < kBuckets / 64; ++j) {
+            const int d = j * 64 + lane;  // of the row
+            const bool in = d >= shift && d < full;
+            const unsigned long long h = in ? row.hist[(long)i * kBuckets + d - shift] : 0;
+            m += in ? ((double)(h >> 48) - (double)(h & kDefMask) * (1.0 / kDefUnit)) * s.factor[d] : 0.0;
         }
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1) m += __shfl_xor(m, d, 64);
@@ -599,7 +681,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams a) {
     const double u = (double)a.uniform[r];
     const double goal = u > 0.0 ? u * kept + kSame * kept : 0.0;
     double total;
-    double acc = scan_d(tid < a.segs ? s.seg_mass[tid] : 0.0, s.wave_d, &total);
+    double acc = block_scan<double>(tid < a.segs ? s.seg_mass[tid] : 0.0, s.wave_d, &total);
     if (tid == 0) s.found_j = kMaxSegs, s.found_i = 0;
     __syncthreads();
     if (tid < a.segs && s.seg_mass[tid] > 0.0) {
@@ -636,7 +718,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams a) {
             sum += y;
         }
     }
-    acc = scan_d(sum, s.wave_d, &total);
+    acc = block_scan<double>(sum, s.wave_d, &total);
     if (tid == 0) s.found_j = kThreads, s.found_i = 0;
     __syncthreads();
     if (sum > 0.0) {
@@ -657,13 +739,23 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams a) {
     }
 }
 
-static size_t hist_offset(int vocab, int rows) {
-    return ((size_t)rows * ceil_div(vocab, kSeg) * sizeof(SegMax) + 255) & ~(size_t)255;
+struct SampleLayout {
+    size_t max, hist, first, list, bytes;
+};
+
+static SampleLayout sample_layout(int vocab, int rows) {
+    const size_t n = (size_t)rows * ceil_div(vocab, kSeg);
+    auto pad = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    SampleLayout l;
+    l.max = 0;
+    l.hist = pad(n * sizeof(SegMax));
+    l.first = l.hist + n * kBuckets * 8;
+    l.list = l.first + n * kBuckets * 2;
+    l.bytes = l.list + n * kSeg * 2;
+    return l;
 }
 
-size_t sample_workspace(int vocab, int rows) {
-    return hist_offset(vocab, rows) + (size_t)rows * ceil_div(vocab, kSeg) * kBuckets * 8;
-}
+size_t sample_workspace(int vocab, int rows) { return sample_layout(vocab, rows).bytes; }
 
 hipError_t launch_sample(const SampleArgs& g, hipStream_t s) {
     SampleParams a;
@@ -678,8 +770,12 @@ hipError_t launch_sample(const SampleArgs& g, hipStream_t s) {
     a.min_p = g.min_p;
     a.uniform = g.uniform;
     a.ids = g.ids;
-    a.seg_max = (SegMax*)g.workspace;
-    a.hist = (unsigned long long*)((char*)g.workspace + hist_offset(g.vocab, g.rows));
+    const SampleLayout l = sample_layout(g.vocab, g.rows);
+    char* w = (char*)g.workspace;
+    a.seg_max = (SegMax*)(w + l.max);
+    a.hist = (unsigned long long*)(w + l.hist);
+    a.first = (uint16_t*)(w + l.first);
+    a.list = (uint16_t*)(w + l.list);
     hipLaunchKernelGGL(sample_segments_kernel, dim3((unsigned)g.rows, (unsigned)a.segs), dim3(kThreads), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
