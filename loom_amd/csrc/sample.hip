@@ -24,7 +24,8 @@ constexpr int kBuckets = 1024;   // 32 nats
 constexpr double kPerNat = 32.0;
 constexpr int kList = 1024;      // a bucket of up to so many tokens is ranked directly
 constexpr int kMaxSegs = 1024;
-constexpr double kFar = 0x1p30;  // |max / T| from which neighbouring floats are over 32 nats apart
+constexpr double kFar = 0x1p35;  // |32 max / T| from which neighbouring floats are over 32 nats apart
+constexpr double kBig = 0x1p15;  // and from which the product's low part counts
 // Masses of the histogram and of single tokens differ by under 2^-39 of the
 // whole; where the definition compares equal sums (equal logits), they must
 // compare equal: a sum within this part of the whole counts as equal.
@@ -40,13 +41,12 @@ struct SegMax {
 };
 
 __device__ __forceinline__ float usable(float x) {  // NaN: never drawn; +inf: the largest finite value
-    if (x != x) return -__builtin_inff();
-    return fminf(x, 3.402823466e38f) + 0.0f;  // (-0 becomes +0)
+    return fminf(fmaxf(x, -__builtin_inff()), 3.402823466e38f);
 }
 
 // Order of values as unsigned integers.
 __device__ __forceinline__ uint32_t key_of(float x) {
-    const uint32_t u = __float_as_uint(x);
+    const uint32_t u = __float_as_uint(x + 0.0f);  // (-0 counts as +0)
     return (u >> 31) ? ~u : u | 0x80000000u;
 }
 
@@ -55,6 +55,23 @@ struct Better {
         return a > b || (a == b && ia < ib);
     }
 };
+
+// Largest over the wave, in every lane: rotations within rows of 16, then the
+// exchanges of rows and halves.
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false)));
+}
+__device__ __forceinline__ float wave_max(float v) {
+    v = dpp_max<0x128>(v);
+    v = dpp_max<0x124>(v);
+    v = dpp_max<0x122>(v);
+    v = dpp_max<0x121>(v);
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 
 // Largest value (lowest index of equal ones) over the workgroup.
 __device__ __forceinline__ void block_best(float& v, int& i, float* sv, int* si) {
@@ -74,16 +91,15 @@ __device__ __forceinline__ void block_best(float& v, int& i, float* sv, int* si)
     __syncthreads();
 }
 
-// z = l / T as a pair, and its bucket on the absolute grid of 1/32 nats.
+// z = l / T on the absolute grid of 1/32 nats: t = 32 z, its bucket b.
 struct Place {
-    double z, lo, b;
+    double t, b;
 };
 
-__device__ __forceinline__ Place place(float l, double inv_t) {
+__device__ __forceinline__ Place place(float l, double per_t) {  // per_t = 32 / T
     Place p;
-    p.z = (double)l * inv_t;
-    p.lo = __builtin_fma((double)l, inv_t, -p.z);
-    p.b = floor(p.z * kPerNat);
+    p.t = (double)l * per_t;
+    p.b = floor(p.t);
     return p;
 }
 
@@ -91,19 +107,25 @@ __device__ __forceinline__ Place place(float l, double inv_t) {
 // it is too far to have a mass).
 __device__ __forceinline__ int bucket_of(const Place& p, const Place& top) {
     const double d = top.b - p.b;
-    if (fabs(top.z) >= kFar) return p.z == top.z ? 0 : kBuckets;
+    if (fabs(top.t) >= kFar) return p.t == top.t ? 0 : kBuckets;
     return d < (double)kBuckets ? (int)d : kBuckets;
 }
 
-// 1 - exp(r) for r in [-1/32, 0] (Taylor; the first term left out is 6e-15).
-__device__ __forceinline__ double deficit(double r) {
-    double y = 1.0 / 720.0;
-    y = __builtin_fma(y, r, 1.0 / 120.0);
-    y = __builtin_fma(y, r, 1.0 / 24.0);
-    y = __builtin_fma(y, r, 1.0 / 6.0);
-    y = __builtin_fma(y, r, 0.5);
-    y = __builtin_fma(y, r, 1.0);
-    return -r * y;
+// What the rounded product t leaves off (counts from |t| = kBig on).
+__device__ __forceinline__ double low_part(float l, double per_t, double t) { return __builtin_fma((double)l, per_t, -t); }
+
+// (1 - exp(r / 32)) * 2^39 as an integer, for r in [-1, 0]: Taylor, the first
+// term left out is under 1.3e-12; the sum with 2^52 leaves the integer in the
+// low bits.
+__device__ __forceinline__ unsigned long long deficit(double r) {
+    constexpr double h = 1.0 / 32.0, u = 0x1p39;
+    double y = -u * h * h * h * h * h / 120.0;
+    y = __builtin_fma(y, r, -u * h * h * h * h / 24.0);
+    y = __builtin_fma(y, r, -u * h * h * h / 6.0);
+    y = __builtin_fma(y, r, -u * h * h / 2.0);
+    y = __builtin_fma(y, r, -u * h);
+    y = __builtin_fma(y, r, 0x1p52);
+    return (unsigned long long)__double_as_longlong(y) & ((1ull << 52) - 1);
 }
 
 // Four consecutive logits of a row at i (i % 4 == 0), -inf past the end.
@@ -149,26 +171,50 @@ struct Filters {
     }
 };
 
+// v of another lane of the wave (CTRL), 0 where there is none or the row is not
+// in ROWS.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T dpp_of(T v) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+    } else {
+        const long long b = __builtin_bit_cast(long long, v);
+        const int lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, false);
+        const int hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
+        return __builtin_bit_cast(T, (long long)(((unsigned long long)(uint32_t)hi << 32) | (uint32_t)lo));
+    }
+}
+
+// Inclusive sums in lane order (row_shr 1, 2, 4, 8, then the rows' last lanes).
+template <typename T>
+__device__ __forceinline__ T row_scan(T v) {
+    v += dpp_of<0x111, 0xf>(v);
+    v += dpp_of<0x112, 0xf>(v);
+    v += dpp_of<0x114, 0xf>(v);
+    v += dpp_of<0x118, 0xf>(v);
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v = row_scan(v);
+    v += dpp_of<0x142, 0xa>(v);
+    v += dpp_of<0x143, 0xc>(v);
+    return v;
+}
+
 // Inclusive sums over the workgroup in thread order, and their total.
 template <typename T>
 __device__ __forceinline__ T block_scan(T v, T* wave_sum, T* total) {
+    static_assert(kThreads == 1024, "one row of lanes scans the waves' sums");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const T o = __shfl_up(v, d, 64);
-        if (lane >= d) v += o;
-    }
+    v = wave_scan(v);
     __syncthreads();
     if (lane == 63) wave_sum[wave] = v;
     __syncthreads();
-    T before = 0, all = 0;
-    for (int w = 0; w < kThreads / 64; ++w) {
-        const T x = wave_sum[w];
-        if (w < wave) before += x;
-        all += x;
-    }
-    *total = all;
-    return v + before;
+    const T all = row_scan(wave_sum[lane & 15]);
+    *total = __shfl(all, 15, 64);
+    const T before = __shfl(all, wave > 0 ? wave - 1 : 0, 64);
+    return wave > 0 ? v + before : v;
 }
 
 // One workgroup per (segment, row): its largest value, its histogram relative
@@ -182,7 +228,7 @@ __global__ __launch_bounds__(kThreads) void sample_segments_kernel(SampleParams 
     __shared__ uint16_t first[kBuckets];
     __shared__ __align__(16) uint16_t list[kSeg];
     __shared__ float sv[kThreads / 64];
-    __shared__ int si[kThreads / 64];
+    __shared__ int si[kThreads / 64], at_s;
     const int tid = threadIdx.x, seg = blockIdx.y;
     const long row = blockIdx.x;
     const float* x = a.logits + row * a.stride;
@@ -194,33 +240,45 @@ __global__ __launch_bounds__(kThreads) void sample_segments_kernel(SampleParams 
     }
     hist[tid] = 0;
     const Filters fl(a, row);
-    float best = -__builtin_inff();
-    int at = 0x7fffffff;
+    float best = l[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int idx = seg * kSeg + 4 * tid + (i >> 2) * 4 * kThreads + (i & 3);
-        if (l[i] > best) best = l[i], at = idx;
-    }
-    block_best(best, at, sv, si);
+    for (int i = 1; i < 8; ++i) best = fmaxf(best, l[i]);
+    best = wave_max(best);
+    if ((tid & 63) == 0) sv[tid >> 6] = best;
+    if (tid == 0) at_s = 0x7fffffff;
+    __syncthreads();
+    best = sv[tid & (kThreads / 64 - 1)];
+    best = wave_max(best);
     const long slot = row * a.segs + seg;
-    if (!(fl.temperature > 0.0f) || best == -__builtin_inff()) {  // greedy, or nothing to draw: the maximum is all
-        if (tid == 0) a.seg_max[slot] = SegMax{best, at, 0};
+    const bool draws = fl.temperature > 0.0f && best > -__builtin_inff();
+    if (!draws) {  // greedy, or nothing to draw: the first of the largest is all
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+            if (l[i] == best) atomicMin(&at_s, seg * kSeg + 4 * tid + (i >> 2) * 4 * kThreads + (i & 3));
+        }
+        __syncthreads();
+        if (tid == 0) a.seg_max[slot] = SegMax{best, at_s, 0};
         return;
     }
-    const double inv_t = 1.0 / (double)fl.temperature;
-    const Place top = place(best, inv_t);
-    const bool far = fabs(top.z) >= kFar;
+    const double per_t = kPerNat / (double)fl.temperature;
+    const Place top = place(best, per_t);
+    const bool far = fabs(top.t) >= kFar, big = fabs(top.t) >= kBig;
     int place_of[8];  // bucket << 16 | place in it
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         place_of[i] = -1;
         if (l[i] == -__builtin_inff()) continue;
-        const Place p = place(l[i], inv_t);
-        const int d = bucket_of(p, top);
+        const Place p = place(l[i], per_t);
+        int d;
+        double r = (p.t - p.b) - 1.0;
+        if (big) {  // (uniform)
+            d = bucket_of(p, top);
+            r = far ? 0.0 : fmin(fmax(r + low_part(l[i], per_t, p.t), -1.0), 0.0);
+        } else {
+            d = (int)(top.b - p.b);
+        }
         if (d >= kBuckets) continue;
-        double r = far ? 0.0 : (p.z - (p.b + 1.0) / kPerNat) + p.lo;
-        r = fmin(fmax(r, -1.0 / kPerNat), 0.0);
-        const unsigned long long old = atomicAdd(&hist[d], (1ull << 48) | (unsigned long long)(deficit(r) * kDefUnit + 0.5));
+        const unsigned long long old = atomicAdd(&hist[d], (1ull << 48) | deficit(r));
         place_of[i] = d << 16 | (int)(old >> 48);
     }
     __syncthreads();
@@ -243,7 +301,7 @@ __global__ __launch_bounds__(kThreads) void sample_segments_kernel(SampleParams 
         __syncthreads();
         if (8 * tid < listed) ((uint4*)(a.list + slot * kSeg))[tid] = ((const uint4*)list)[tid];
     }
-    if (tid == 0) a.seg_max[slot] = SegMax{best, at, listed};
+    if (tid == 0) a.seg_max[slot] = SegMax{best, seg * kSeg, listed};
 }
 
 // What a row keeps: buckets up to `bucket`, and of those the tokens ranked at
@@ -278,7 +336,7 @@ struct Row {
     const float* x;
     int vocab, segs;
     bool vec;
-    double inv_t;
+    double inv_t, per_t;  // 1 / T, 32 / T
     float max;
     Place top;
     const SegMax* seg_max;
@@ -292,7 +350,7 @@ struct Row {
     __device__ __forceinline__ unsigned long long fixed(float l) const {
         return (unsigned long long)(weight(l) * kMassUnit + 0.5);
     }
-    __device__ __forceinline__ int bucket(float l) const { return bucket_of(place(l, inv_t), top); }
+    __device__ __forceinline__ int bucket(float l) const { return bucket_of(place(l, per_t), top); }
 
     // f(value, key, index) for the row's tokens in buckets b0..b1 that the cut
     // keeps, from the segments' lists: a wave a segment
@@ -527,6 +585,71 @@ __device__ double resolve(const Row& row, PickShared& s, int b0, int b1, long lo
     return above;
 }
 
+// The whole of a row whose filters leave only tokens of buckets 0..b, n <=
+// kFew of them: each ranked against the others, then summed by index.
+// `whole` is the mass that top-p refers to where top-k is off.
+constexpr int kFew = 256;
+
+__device__ void pick_few(const Row& row, PickShared& s, int b, int n, const Filters& fl, bool kon, double whole,
+                         float uniform, int* id) {
+    const int tid = threadIdx.x;
+    if (tid == 0) {
+        s.n = 0;
+        s.lo_ord = s.hi_ord = 0;  // masses of the first k, and of what is kept
+        s.found_i = -1;
+        s.found_j = 0x7fffffff;
+    }
+    __syncthreads();
+    const Cut all{kBuckets - 1, 0u, 0x7fffffff};
+    row.each(s, 0, b, all, [&](float l, uint32_t k, int idx) {
+        const int at = atomicAdd(&s.n, 1);
+        if (at < kFew) s.list_key[at] = k, s.list_idx[at] = idx, s.list_w[at] = row.fixed(l);
+    });
+    __syncthreads();
+    n = s.n < kFew ? s.n : kFew;
+    const bool mine = tid < n;
+    uint32_t key = 0;
+    int idx = 0, rank = 0;
+    unsigned long long w = 0, before = 0;
+    const int k = kon ? fl.top_k : 0x7fffffff;
+    if (mine) {
+        key = s.list_key[tid], idx = s.list_idx[tid], w = s.list_w[tid];
+        for (int j = 0; j < n; ++j) {
+            const uint32_t kj = s.list_key[j];
+            const bool first = kj > key || (kj == key && s.list_idx[j] < idx);
+            rank += first;
+            before += first ? s.list_w[j] : 0;
+        }
+        if (rank < k) atomicAdd(&s.lo_ord, w);
+    }
+    __syncthreads();
+    const double of = kon ? (double)s.lo_ord * (1.0 / kMassUnit) : whole;
+    const double p = (double)fl.top_p, mp = fmin((double)fl.min_p, 1.0);
+    bool keep = mine && rank < k;
+    if (keep && rank > 0) {
+        if (p < 1.0) keep = (double)before * (1.0 / kMassUnit) < p * of - kSame * of;
+        if (mp > 0.0) {
+            const uint32_t v = (key >> 31) ? (key & 0x7fffffffu) : ~key;
+            keep = keep && row.weight(__uint_as_float(v)) >= mp;
+        }
+    }
+    if (mine) s.list_w[tid] = keep ? w : 0;
+    if (keep) {
+        atomicAdd(&s.hi_ord, w);
+        if (w > 0) atomicMax(&s.found_i, idx);
+    }
+    __syncthreads();
+    const double kept = (double)s.hi_ord, u = (double)uniform;
+    const double goal = u > 0.0 ? u * kept + kSame * kept : 0.0;
+    if (keep && w > 0) {
+        unsigned long long upto = 0;
+        for (int j = 0; j < n; ++j) upto += s.list_idx[j] <= idx ? s.list_w[j] : 0;
+        if ((double)upto > goal) atomicMin(&s.found_j, idx);
+    }
+    __syncthreads();
+    if (tid == 0) *id = s.found_j != 0x7fffffff ? s.found_j : s.found_i;
+}
+
 // First bucket whose running count (mass) reaches the target.
 template <typename F>
 __device__ __forceinline__ int first_bucket(PickShared& s, F reached) {
@@ -566,17 +689,18 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams a) {
     }
     row.inv_t = 1.0 / (double)fl.temperature;
     row.max = best;
-    row.top = place(best, row.inv_t);
+    row.per_t = kPerNat / (double)fl.temperature;
+    row.top = place(best, row.per_t);
     row.seg_max = sm;
     row.hist = a.hist + r * a.segs * kBuckets;
     row.first = a.first + r * a.segs * kBuckets;
     row.list = a.list + r * a.segs * kSeg;
-    const bool far = fabs(row.top.z) >= kFar;
+    const bool far = fabs(row.top.t) >= kFar;
 
     // the segments' histograms on the row's grid
     for (int i = tid; i < a.segs; i += kThreads) {
         const float v = sm[i].value;
-        s.shift[i] = v == -__builtin_inff() ? kBuckets : bucket_of(place(v, row.inv_t), row.top);
+        s.shift[i] = v == -__builtin_inff() ? kBuckets : bucket_of(place(v, row.per_t), row.top);
     }
     __syncthreads();
     unsigned long long def = 0;
@@ -588,8 +712,10 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams a) {
         cnt += (int)(h >> 48);
         def += h & kDefMask;
     }
-    const double edge = far ? (tid == 0 ? 0.0 : -1e30) : ((row.top.b - tid + 1.0) / kPerNat - row.top.z) - row.top.lo;
-    const double factor = exp(edge);
+    // a bucket's upper edge under the maximum, in 1/32 nats
+    const double edge = far ? (tid == 0 ? 0.0 : -1e30)
+                            : ((row.top.b - tid + 1.0) - row.top.t) - low_part(best, row.per_t, row.top.t);
+    const double factor = exp(edge / kPerNat);
     s.factor[tid] = factor;
     long long tokens;
     double whole;
@@ -607,59 +733,77 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleParams a) {
     auto mass_before = [&](int b) { return b > 0 ? s.mass[b - 1] : 0.0; };
 
     const long long k = fl.top_k;
-    if (k > 0 && k < tokens) {
-        const int b = first_bucket(s, [&](int i) { return s.count[i] >= k; });
-        const long long nb = s.count[b] - count_before(b), take = k - count_before(b);
-        if (take == nb) {
-            cut.bucket = b;
-            full = b + 1;
-            kept = s.mass[b];
-        } else {
-            kept = resolve(row, s, b, b, nb, take, 0.0, mass_before(b), &cut);
-            full = b;
+    if (fl.any(a.vocab)) {
+        // the last bucket that any filter leaves tokens in (top-p of top-k needs
+        // all of the first k)
+        const bool kon = k > 0 && k < tokens;
+        const double target = (double)fl.top_p * whole - kSame * whole, least = fmin((double)fl.min_p, 1.0) * (1.0 - 1e-9);
+        const int b = first_bucket(s, [&](int i) {
+            return (kon && s.count[i] >= k) || (!kon && fl.top_p < 1.0f && s.count[i] > 0 && s.mass[i] >= target) ||
+                   (!(kon && fl.top_p < 1.0f) && fl.min_p > 0.0f && s.factor[i] < least);
+        });
+        if (s.count[b] <= kFew) {
+            pick_few(row, s, b, s.count[b], fl, kon, whole, a.uniform[r], a.ids + r);
+            return;
         }
     }
+    // top-k, top-p, min-p, each narrowing what the one before has left; at most
+    // one place in the buckets to resolve each (one loop, so that the code of it
+    // is there once: a row's kernel runs through its code a single time)
     const double p = (double)fl.top_p;
-    if (p < 1.0) {
-        const double target = p > 0.0 ? p * kept - kSame * kept : 0.0;
-        int b = first_bucket(s, [&](int i) { return s.count[i] > 0 && s.mass[i] >= target; });
-        if (b > cut.bucket) b = cut.bucket;
-        const long long nb = s.count[b] - count_before(b);
-        kept = resolve(row, s, b, b, nb, 0, target, mass_before(b), &cut);
-        full = b;
-    }
-    double mp = (double)fl.min_p;
-    if (mp > 1.0) mp = 1.0;
-    if (mp > 0.0) {
-        // buckets that are neither whole above min_p nor whole below it
-        const int b0 = first_bucket(s, [&](int i) { return s.factor[i] * exp(-1.0 / kPerNat) < mp * (1.0 + 1e-9); });
-        int b1 = first_bucket(s, [&](int i) { return s.factor[i] < mp * (1.0 - 1e-9); });
-        if (b1 > b0) --b1;
-        if (b1 > cut.bucket) b1 = cut.bucket;
-        if (b0 <= b1) {
-            int mine = 0, of = 0;
-            row.each(s, b0, b1, cut, [&](float l, uint32_t, int) {
-                ++of;
-                mine += row.weight(l) >= mp;
-            });
-            long long got, all;
-            (void)block_scan<long long>(mine, s.wave_i, &got);
-            (void)block_scan<long long>(of, s.wave_i, &all);
+    const double mp = fmin((double)fl.min_p, 1.0);
+#pragma unroll 1
+    for (int stage = 0; stage < 3; ++stage) {
+        int b0 = 0, b1 = 0;
+        long long take = 0;
+        double target = 0.0;
+        if (stage == 0) {
+            if (!(k > 0 && k < tokens)) continue;
+            b0 = b1 = first_bucket(s, [&](int i) { return s.count[i] >= k; });
+            take = k - count_before(b0);
+            if (take == s.count[b0] - count_before(b0)) {
+                cut.bucket = b0;
+                full = b0 + 1;
+                kept = s.mass[b0];
+                continue;
+            }
+        } else if (stage == 1) {
+            if (!(p < 1.0)) continue;
+            target = p > 0.0 ? p * kept - kSame * kept : 0.0;
+            b0 = first_bucket(s, [&](int i) { return s.count[i] > 0 && s.mass[i] >= target; });
+            if (b0 > cut.bucket) b0 = cut.bucket;
+            b1 = b0;
+        } else {
+            if (!(mp > 0.0)) continue;
+            // buckets that are neither whole above min_p nor whole below it
+            b0 = first_bucket(s, [&](int i) { return s.factor[i] * 0.969233234476344 < mp * (1.0 + 1e-9); });  // e^(-1/32)
+            b1 = first_bucket(s, [&](int i) { return s.factor[i] < mp * (1.0 - 1e-9); });
+            if (b1 > b0) --b1;
+            if (b1 > cut.bucket) b1 = cut.bucket;
+            if (b0 > b1) continue;
+            long long mine = 0, got, all;
+            row.each(s, b0, b1, cut, [&](float l, uint32_t, int) { mine += 0x100000000ll + (row.weight(l) >= mp); });
+            (void)block_scan<long long>(mine, s.wave_i, &all);
+            got = all & 0xffffffffll;
+            all >>= 32;
             if (got == 0 && b0 > 0) {
                 cut.bucket = b0 - 1;
                 full = b0;
                 kept = mass_before(b0);
-            } else if (got == all) {
+                continue;
+            }
+            if (got == all) {
                 if (b1 < cut.bucket) {
                     cut.bucket = b1;
                     full = b1 + 1;
                     kept = mass_before(b1 + 1);
                 }
-            } else {
-                kept = resolve(row, s, b0, b1, s.count[b1] - count_before(b0), got, 0.0, mass_before(b0), &cut);
-                full = b0;
+                continue;
             }
+            take = got;
         }
+        kept = resolve(row, s, b0, b1, s.count[b1] - count_before(b0), take, target, mass_before(b0), &cut);
+        full = b0;
     }
 
     // the segment where the kept mass passes u of the whole
