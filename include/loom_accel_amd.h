@@ -489,6 +489,23 @@ int loom_amd_paged_attention(const loom_amd_kv_pages* cache, const int32_t* page
                              int heads, int64_t q_stride, float scale, int max_context, void* out,
                              int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
 
+/* One block forward on rows of many requests, in place on x (DEVICE, rows x
+ * hidden fp32), over a paged cache instead of the block's ring: the stages of
+ * loom_amd_block_forward, with each row at its own position, its K and V
+ * appended to the cache (loom_amd_kv_append, fp32 rows) and attention over it
+ * (loom_amd_paged_attention: 8-bit keys and values, fp32 sums; the ring's
+ * attention is fp64 over fp32 rows).  pages, row_start, positions and slots as
+ * a plan gives them.  The cache has the block's kv_heads and head_dim.  Rows
+ * without a place have no attention; they are written like the others, and mean
+ * nothing.  Independent of the block's own positions and ring.  May grow the
+ * block's workspace (synchronizing the device) when rows, requests or
+ * max_context exceed earlier calls: make the largest call once before a
+ * capture.  Calls on one block must not overlap. */
+int loom_amd_block_forward_paged(loom_amd_block* b, float* x, int rows, const loom_amd_kv_pages* cache,
+                                 const int32_t* pages, int requests, int max_pages, const int32_t* row_start,
+                                 const int32_t* positions, const int32_t* slots, int max_context,
+                                 const loom_amd_block_taps* taps, void* stream);
+
 /* ---- sampling ---------------------------------------------------------- */
 
 #define LOOM_AMD_SAMPLE_MAX_VOCAB 8388608

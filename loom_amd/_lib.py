@@ -154,6 +154,8 @@ SIGNATURES = {
     "loom_amd_paged_attention_workspace": (i32, [i32, i32, i32, i32, i32, i32, C.POINTER(sz)]),
     "loom_amd_paged_attention": (i32, [C.POINTER(KvPages), P, i32, i32, P, P, P, i32, i32, i32, i64, f32,
                                        i32, P, i64, P, sz, P]),
+    "loom_amd_block_forward_paged": (i32, [P, P, i32, C.POINTER(KvPages), P, i32, i32, P, P, P, i32,
+                                           C.POINTER(BlockTaps), P]),
     "loom_amd_sample_workspace": (i32, [i32, i32, C.POINTER(sz)]),
     "loom_amd_sample": (i32, [P, i64, i32, i32, P, P, P, P, P, P, P, sz, P]),
 }

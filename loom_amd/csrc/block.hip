@@ -391,6 +391,10 @@ constexpr int kRopeMaxHalf = 128;  // head_dim <= 256
 // With per-head norms the workgroup first forms the norm factor of every Q
 // and K head of its row (one thread per head, the dimension-order chain) into
 // LDS.
+//
+// ROWS: row t stands at position pos0[t] of a request (below 0: no place, at
+// position 0), and its K and V go to row t of cache_k and cache_v.
+template <bool ROWS>
 __global__ __launch_bounds__(256) void qkv_rope_kernel(
     const int32_t* __restrict__ acc, const float* __restrict__ amax, float sq, float sk, float sv,
     const float* __restrict__ bq, const float* __restrict__ bk, const float* __restrict__ bv, int batch,
@@ -403,8 +407,8 @@ __global__ __launch_bounds__(256) void qkv_rope_kernel(
     const int qp = heads * half, kp = kv_heads * half;
     const int per_row = qp + kp + kv_dim;
     const int row = blockIdx.x;  // token row b*seq + s
-    const int b = row / seq, s = row % seq;
-    const int base = *pos0;
+    const int b = ROWS ? 0 : row / seq, s = ROWS ? 0 : row % seq;
+    const int base = ROWS ? max(pos0[row], 0) : *pos0;
     const int pos = base + s;
     for (int d = threadIdx.x; d < half; d += blockDim.x) rope_angle(pos, d, hd, theta, &rc[d], &rs[d]);
     const int32_t* ar = acc + (size_t)row * (q_dim + 2 * kv_dim);
@@ -424,10 +428,10 @@ __global__ __launch_bounds__(256) void qkv_rope_kernel(
     __syncthreads();
     cache_k += (size_t)b * msl * kv_dim;
     cache_v += (size_t)b * msl * kv_dim;
-    const bool latest = pos + msl >= base + seq;
+    const bool latest = ROWS || pos + msl >= base + seq;
     double* qr = q + (size_t)row * q_dim;
-    float* kr = cache_k + (size_t)(pos % msl) * kv_dim;
-    float* vr = cache_v + (size_t)(pos % msl) * kv_dim;
+    float* kr = cache_k + (size_t)(ROWS ? row : pos % msl) * kv_dim;
+    float* vr = cache_v + (size_t)(ROWS ? row : pos % msl) * kv_dim;
     for (int r = threadIdx.x + blockIdx.y * blockDim.x; r < per_row; r += blockDim.x * gridDim.y) {
         if (r < qp) {
             const int h = r / half, d = r % half;
@@ -460,9 +464,24 @@ hipError_t launch_qkv_rope(const int32_t* acc, const float* amax, float sq, floa
     if (theta <= 0.0) theta = 10000.0;
     const int per_row = heads * (hd / 2) + kv_heads * (hd / 2) + kv_heads * hd;
     const int parts = rows >= 256 ? 1 : ceil_div(per_row, 256);
-    hipLaunchKernelGGL(qkv_rope_kernel, dim3((unsigned)rows, parts), dim3(256), 0, s, acc, amax, sq,
+    hipLaunchKernelGGL(qkv_rope_kernel<false>, dim3((unsigned)rows, parts), dim3(256), 0, s, acc, amax, sq,
                        sk, sv, bq, bk, bv, batch, seq, pos0, msl, heads, kv_heads, hd, theta, q,
                        cache_k, cache_v, qk);
+    return hipGetLastError();
+}
+
+hipError_t launch_qkv_rope_rows(const int32_t* acc, const float* amax, float sq, float sk, float sv,
+                                const float* bq, const float* bk, const float* bv, int rows,
+                                const int* positions, int heads, int kv_heads, int hd, double theta,
+                                double* q, float* k, float* v, hipStream_t s, const QkNorm& qk) {
+    if (rows <= 0) return hipSuccess;
+    if (hd % 2 != 0 || hd / 2 > kRopeMaxHalf) return hipErrorInvalidValue;
+    if ((qk.q || qk.k) && heads + kv_heads > kQkNormMaxHeads) return hipErrorInvalidValue;
+    if (theta <= 0.0) theta = 10000.0;
+    const int per_row = heads * (hd / 2) + kv_heads * (hd / 2) + kv_heads * hd;
+    const int parts = rows >= 256 ? 1 : ceil_div(per_row, 256);
+    hipLaunchKernelGGL(qkv_rope_kernel<true>, dim3((unsigned)rows, parts), dim3(256), 0, s, acc, amax, sq,
+                       sk, sv, bq, bk, bv, 1, rows, positions, 1, heads, kv_heads, hd, theta, q, k, v, qk);
     return hipGetLastError();
 }
 

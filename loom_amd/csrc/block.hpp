@@ -47,6 +47,13 @@ hipError_t launch_qkv_rope(const int32_t* acc, const float* amax, float sq, floa
                            double* q, float* cache_k, float* cache_v, hipStream_t s,
                            const QkNorm& qk = QkNorm{});
 
+// The same for rows that each stand at a position of their own (below 0: at 0):
+// K and V rows dense (rows x kv_dim) instead of into a ring.
+hipError_t launch_qkv_rope_rows(const int32_t* acc, const float* amax, float sq, float sk, float sv,
+                                const float* bq, const float* bk, const float* bv, int rows,
+                                const int* positions, int heads, int kv_heads, int hd, double theta,
+                                double* q, float* k, float* v, hipStream_t s, const QkNorm& qk = QkNorm{});
+
 // Causal attention of batch x seq queries at positions *pos0 + s over each
 // sequence's ring cache.  span >= *pos0 + seq must hold (LDS holds span
 // scores) and span <= msl.  Up to kSplitMaxRows query rows take the split

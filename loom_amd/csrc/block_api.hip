@@ -1,6 +1,7 @@
 // block_api.hip -- loom_amd_block_* and loom_amd_model_* entry points
 // (include/loom_accel_amd.h): one BitNet decoder block, and the greedy
 // decode loop of a stack of them, device-resident end to end.
+#include <math.h>
 #include <stdlib.h>
 #include <string.h>
 
@@ -11,6 +12,7 @@
 #include "block.hpp"
 #include "lamd.hpp"
 #include "loom_accel_amd.h"
+#include "paged.hpp"
 
 namespace lamd {
 
@@ -60,7 +62,8 @@ struct Workspace {
     double* totals = nullptr;  // rows x fp64: strict ordered sums of squares (many rows)
 };
 
-static size_t workspace_layout(const BlockDev& B, int rows, Workspace* W, char* base) {
+// paged: no scores of the ring's attention.
+static size_t workspace_layout(const BlockDev& B, int rows, Workspace* W, char* base, bool paged = false) {
     Layout L;
     const size_t r = (size_t)rows;
     const size_t o_xq = L.take(r * pad_cols(B.hidden));
@@ -72,7 +75,7 @@ static size_t workspace_layout(const BlockDev& B, int rows, Workspace* W, char* 
     const size_t sc_small = attention_scratch_bytes(rows < kSplitMaxRows ? rows : kSplitMaxRows,
                                                     B.heads, B.hd, B.span(), B.strict, B.attn_qt);
     const size_t sc_big = attention_scratch_bytes(rows, B.heads, B.hd, B.span(), B.strict, B.attn_qt);
-    const size_t o_sc = L.take(sc_small > sc_big ? sc_small : sc_big);
+    const size_t o_sc = L.take(paged ? 0 : (sc_small > sc_big ? sc_small : sc_big));
     const size_t o_aq = L.take(r * pad_cols(B.q_dim));
     const size_t o_am2 = L.take(r * 4);
     const size_t o_xs2 = L.take(r * 4);
@@ -109,12 +112,12 @@ static void free_workspace(Workspace* W) {
     *W = Workspace{};
 }
 
-static int alloc_workspace(const BlockDev& B, int rows, Workspace* W) {
-    const size_t bytes = workspace_layout(B, rows, nullptr, nullptr);
+static int alloc_workspace(const BlockDev& B, int rows, Workspace* W, bool paged = false) {
+    const size_t bytes = workspace_layout(B, rows, nullptr, nullptr, paged);
     void* p = nullptr;
     hipError_t e = hipMalloc(&p, bytes);
     if (e != hipSuccess) return fail_hip("block workspace", e);
-    workspace_layout(B, rows, W, (char*)p);
+    workspace_layout(B, rows, W, (char*)p, paged);
     return 0;
 }
 
@@ -322,14 +325,23 @@ static hipError_t tap_rows(int8_t* dst, const int8_t* src, int ld, int n, int ro
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// Enqueues one block forward on x (rows = batch*seq) at device position *pos.
+// Rows of many requests over a paged cache instead of the block's ring.
+struct PagedRows {
+    PagedAttn attn;  // q, out, rows and workspace are filled in by the block
+    const int32_t* slots;
+    float *k, *v;  // rows x kv_dim
+};
+
+// Enqueues one block forward on x (rows = batch*seq) at device position *pos
+// (paged: batch = 1, seq = rows, each row at its own position).
 // Few rows take the decode path: each row norm runs inside the matmul that
 // consumes it (launch_matmul_norm).  Taps never change the path: every stage
 // writes its tap from the kernel that computes it (workgroup 0 of a
 // norm-fused matmul, the chunk-0 workgroups of the fused decode attention) or
 // by a copy of the workspace it leaves behind.
 static int block_forward_dev(const BlockDev& B, const Workspace& W, float* x, int batch, int seq,
-                             const int* pos, const loom_amd_block_taps* taps, hipStream_t s) {
+                             const int* pos, const loom_amd_block_taps* taps, hipStream_t s,
+                             const PagedRows* paged = nullptr) {
     const int R = batch * seq;
     const int ldh = pad_cols(B.hidden), ldqd = pad_cols(B.q_dim), ldi = pad_cols(B.inter);
     const double rms_eps = B.norm_eps > 0 ? B.norm_eps : 1e-6;   // RMSNormForwardPolymorphic
@@ -366,7 +378,23 @@ static int block_forward_dev(const BlockDev& B, const Workspace& W, float* x, in
         }
         TAP(tap_copy(T.amax1, W.amax, (size_t)R * 4, s));
     }
-    if (B.fuse_rope && batch <= kSplitMaxRows && attention_rope_ok(seq, B.hd, B.strict, B.span())) {
+    if (paged) {
+        e = launch_qkv_rope_rows(W.acc, W.amax, B.sq, B.sk, B.sv, B.bq, B.bk, B.bv, R, paged->attn.positions,
+                                 B.heads, B.kv_heads, B.hd, B.theta, W.q, paged->k, paged->v, s, B.qk);
+        if (e != hipSuccess) return fail_hip("block qkv rope", e);
+        TAP(tap_copy(T.q, W.q, (size_t)R * B.q_dim * 8, s));
+        e = launch_kv_append(paged->attn.c, paged->k, paged->v, ROW_F32, R, B.kv_dim, B.kv_dim, paged->slots, s);
+        if (e != hipSuccess) return fail_hip("block kv append", e);
+        PagedAttn a = paged->attn;
+        a.q = W.q;
+        a.out = W.attn;
+        a.type = ROW_F64;
+        a.rows = R;
+        a.heads = B.heads;
+        a.q_stride = a.out_stride = B.q_dim;
+        e = launch_paged_attn(a, s);
+        if (e != hipSuccess) return fail_hip("block attention", e);
+    } else if (B.fuse_rope && batch <= kSplitMaxRows && attention_rope_ok(seq, B.hd, B.strict, B.span())) {
         // decode: the Q/K/V epilogue runs inside the attention launch
         e = launch_attention_rope(W.acc, W.amax, B.sq, B.sk, B.sv, B.bq, B.bk, B.bv, B.theta, batch, pos,
                                   B.msl, B.span(), B.heads, B.kv_heads, B.hd, B.strict, B.cache_k,
@@ -484,6 +512,10 @@ using namespace lamd;
 struct loom_amd_block {
     BlockDev dev;
     Workspace ws;
+    // forward_paged: intermediates, and k, v rows and attention's workspace
+    Workspace paged_ws;
+    void* paged_extra = nullptr;
+    size_t paged_extra_bytes = 0;
     int* pos = nullptr;  // device
     int shadow = 0;      // host copy of the KV position
     int warm_batch = 0;  // sequences the warm cache holds (batch of the calls that filled it)
@@ -560,6 +592,8 @@ void loom_amd_block_release(loom_amd_block* b) {
     DeviceGuard guard(b->dev.device);
     (void)hipDeviceSynchronize();
     free_workspace(&b->ws);
+    free_workspace(&b->paged_ws);
+    if (b->paged_extra) (void)hipFree(b->paged_extra);
     free_block(&b->dev);
     if (b->pos) (void)hipFree(b->pos);
     delete b;
@@ -604,6 +638,59 @@ int loom_amd_block_forward(loom_amd_block* b, float* x, int batch, int seq,
     b->shadow = base + seq;
     b->warm_batch = batch;
     return 0;
+}
+
+int loom_amd_block_forward_paged(loom_amd_block* b, float* x, int rows, const loom_amd_kv_pages* cache,
+                                 const int32_t* pages, int requests, int max_pages, const int32_t* row_start,
+                                 const int32_t* positions, const int32_t* slots, int max_context,
+                                 const loom_amd_block_taps* taps, void* stream) {
+    if (!b) return fail("block is null");
+    const BlockDev& B = b->dev;
+    PagedRows pr{};
+    if (check_kv_pages(cache, &pr.attn.c)) return -1;
+    if (pr.attn.c.kv_heads != B.kv_heads || pr.attn.c.hd != B.hd) {
+        return fail("cache of " + std::to_string(pr.attn.c.kv_heads) + " heads of " + std::to_string(pr.attn.c.hd) +
+                    ", block has " + std::to_string(B.kv_heads) + " of " + std::to_string(B.hd));
+    }
+    if (check_paged_rows(pr.attn.c, requests, max_pages, rows, B.heads, max_context)) return -1;
+    if (rows == 0) return 0;
+    if (!x || !pages || !row_start || !positions || !slots) return fail("null buffer");
+    DeviceGuard guard(B.device);
+    hipStream_t s = (hipStream_t)stream;
+    const size_t kv = ((size_t)rows * B.kv_dim * 4 + 255) & ~(size_t)255;
+    const size_t extra = 2 * kv + paged_attn_workspace(rows, B.heads, B.kv_heads, B.hd, requests, max_context);
+    if (b->paged_ws.rows < rows || b->paged_extra_bytes < extra) {
+        hipError_t e = hipDeviceSynchronize();  // queued calls may still use the old workspace
+        if (e != hipSuccess) return fail_hip("block workspace", e);
+        if (b->paged_ws.rows < rows) {
+            free_workspace(&b->paged_ws);
+            if (alloc_workspace(B, rows, &b->paged_ws, true)) return -1;
+        }
+        if (b->paged_extra_bytes < extra) {
+            if (b->paged_extra) (void)hipFree(b->paged_extra);
+            b->paged_extra = nullptr;
+            b->paged_extra_bytes = 0;
+            e = hipMalloc(&b->paged_extra, extra);
+            if (e != hipSuccess) return fail_hip("block workspace", e);
+            b->paged_extra_bytes = extra;
+        }
+        // a row of no request has no attention: it goes on with zeros, not with what was here
+        e = hipMemset(b->paged_ws.attn, 0, (size_t)b->paged_ws.rows * B.q_dim * 8);
+        if (e == hipSuccess) e = hipDeviceSynchronize();
+        if (e != hipSuccess) return fail_hip("block workspace", e);
+    }
+    pr.attn.table = pages;
+    pr.attn.max_pages = max_pages;
+    pr.attn.requests = requests;
+    pr.attn.row_start = row_start;
+    pr.attn.positions = positions;
+    pr.attn.scale = (float)(1.0 / sqrt((double)B.hd));
+    pr.attn.max_context = max_context;
+    pr.attn.workspace = (char*)b->paged_extra + 2 * kv;
+    pr.slots = slots;
+    pr.k = (float*)b->paged_extra;
+    pr.v = (float*)((char*)b->paged_extra + kv);
+    return block_forward_dev(B, b->paged_ws, x, 1, rows, nullptr, taps, s, &pr);
 }
 
 int loom_amd_block_kv_offset(const loom_amd_block* b) { return b ? b->shadow : -1; }

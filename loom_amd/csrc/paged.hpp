@@ -16,6 +16,7 @@
 #pragma once
 
 #include "lamd.hpp"
+#include "loom_accel_amd.h"
 
 namespace lamd {
 
@@ -85,6 +86,10 @@ struct PagedAttn {
 };
 size_t paged_attn_workspace(int rows, int heads, int kv_heads, int hd, int requests, int max_context);
 hipError_t launch_paged_attn(const PagedAttn& a, hipStream_t s);
+
+// Checks of the entry points (paged_api.hip): 0, or -1 with the message set.
+int check_kv_pages(const loom_amd_kv_pages* c, KvPages* out);
+int check_paged_rows(const KvPages& c, int requests, int max_pages, int rows, int heads, int max_context);
 
 struct SampleArgs {
     const float* logits;

@@ -25,7 +25,7 @@ static int check_table(const loom_amd_page_table* t, PageTables* out) {
     return 0;
 }
 
-static int check_cache(const loom_amd_kv_pages* c, KvPages* out) {
+int check_kv_pages(const loom_amd_kv_pages* c, KvPages* out) {
     if (!c) return fail("kv pages are null");
     if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail("kv pages: null buffer");
     if (c->num_pages <= 0 || c->kv_heads <= 0) return fail("kv pages: num_pages and kv_heads must be positive");
@@ -35,6 +35,22 @@ static int check_cache(const loom_amd_kv_pages* c, KvPages* out) {
     if ((long)c->num_pages * c->page_size > 0x7fffffffl) return fail("kv pages: more than 2^31 - 1 tokens");
     if (((uintptr_t)c->k & 15) || ((uintptr_t)c->v & 15)) return fail("kv pages: codes must be 16-byte aligned");
     *out = KvPages{c->k, c->v, c->k_scale, c->v_scale, c->num_pages, c->page_size, c->kv_heads, c->head_dim};
+    return 0;
+}
+
+static int check_attention(int rows, int heads, int kv_heads, int requests) {
+    if (rows < 0 || heads <= 0 || kv_heads <= 0 || requests <= 0) return fail("bad shape");
+    if (heads % kv_heads != 0) return fail("kv_heads must divide heads");
+    if ((int64_t)rows * heads > 0x7fffffff) return fail("rows * heads exceeds 2^31 - 1");
+    return 0;
+}
+
+int check_paged_rows(const KvPages& c, int requests, int max_pages, int rows, int heads, int max_context) {
+    if (check_attention(rows, heads, c.kv_heads, requests)) return -1;
+    if (max_pages <= 0 || (int64_t)max_pages * c.page > 0x7fffffff) return fail("bad max_pages");
+    if (max_context < 0 || max_context > max_pages * c.page) {
+        return fail("max_context must be within max_pages * page_size");
+    }
     return 0;
 }
 
@@ -75,7 +91,7 @@ int loom_amd_page_table_release(const loom_amd_page_table* table, const uint8_t*
 int loom_amd_kv_append(const loom_amd_kv_pages* cache, const void* k, const void* v, int type, int rows,
                        int64_t k_stride, int64_t v_stride, const int32_t* slots, void* stream) {
     KvPages c;
-    if (check_cache(cache, &c)) return -1;
+    if (check_kv_pages(cache, &c)) return -1;
     if (type != LOOM_AMD_ROW_F32 && type != LOOM_AMD_ROW_BF16) return fail("rows of keys and values are fp32 or bf16");
     if (rows < 0) return fail("bad shape");
     if (rows == 0) return 0;
@@ -89,20 +105,13 @@ int loom_amd_kv_append(const loom_amd_kv_pages* cache, const void* k, const void
 int loom_amd_kv_read(const loom_amd_kv_pages* cache, const int32_t* slots, int rows, float* k, float* v,
                      void* stream) {
     KvPages c;
-    if (check_cache(cache, &c)) return -1;
+    if (check_kv_pages(cache, &c)) return -1;
     if (rows < 0) return fail("bad shape");
     if (rows == 0) return 0;
     if (!slots || !k || !v) return fail("null buffer");
     if (((uintptr_t)k & 15) || ((uintptr_t)v & 15)) return fail("outputs of kv_read must be 16-byte aligned");
     hipError_t e = launch_kv_read(c, slots, rows, k, v, (hipStream_t)stream);
     return e == hipSuccess ? 0 : fail_hip("kv_read", e);
-}
-
-static int check_attention(int rows, int heads, int kv_heads, int requests) {
-    if (rows < 0 || heads <= 0 || kv_heads <= 0 || requests <= 0) return fail("bad shape");
-    if (heads % kv_heads != 0) return fail("kv_heads must divide heads");
-    if ((int64_t)rows * heads > 0x7fffffff) return fail("rows * heads exceeds 2^31 - 1");
-    return 0;
 }
 
 int loom_amd_paged_attention_workspace(int rows, int heads, int kv_heads, int head_dim, int requests,
@@ -121,14 +130,10 @@ int loom_amd_paged_attention(const loom_amd_kv_pages* cache, const int32_t* page
                              int heads, int64_t q_stride, float scale, int max_context, void* out,
                              int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
     KvPages c;
-    if (check_cache(cache, &c)) return -1;
-    if (check_attention(rows, heads, c.kv_heads, requests)) return -1;
+    if (check_kv_pages(cache, &c)) return -1;
+    if (check_paged_rows(c, requests, max_pages, rows, heads, max_context)) return -1;
     if (type != LOOM_AMD_ROW_F32 && type != LOOM_AMD_ROW_BF16 && type != LOOM_AMD_ROW_F64) {
         return fail("rows of queries are fp32, bf16 or fp64");
-    }
-    if (max_pages <= 0 || (int64_t)max_pages * c.page > 0x7fffffff) return fail("bad max_pages");
-    if (max_context < 0 || max_context > max_pages * c.page) {
-        return fail("max_context must be within max_pages * page_size");
     }
     if (!isfinite(scale)) return fail("scale must be finite");
     if (rows == 0) return 0;

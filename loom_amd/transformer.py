@@ -9,6 +9,8 @@ forwardOnCPUNormal block body                          ``BitNetBlock.forward``
   ternary MHA (mha.go:204-371), residual, RMSNorm,
   packed ternary SwiGLU, residual
 KVOffset / mhaPrepareKVForForward (mha_layout.go:62)   ``BitNetBlock.kv_offset``
+(none: many requests over a paged 8-bit cache)         ``BitNetBlock.forward_paged``
+(none: sampling beyond the greedy pick)                ``sample``
 Transformer.Generate greedy (transformer.go:330-520)   ``Transformer.generate``
   prefill: TokensToTensor + ForwardFull + ApplyLMHead  ``Transformer.prefill``
   decode: getEmbedding + forwardOne + ApplyLMHead +    ``Transformer.decode``
@@ -177,26 +179,57 @@ class BitNetBlock:
             batch, seq = 1, batch * seq
         if x.shape[-1] != self.cfg.hidden:
             raise ValueError(f"hidden is {x.shape[-1]}, block expects {self.cfg.hidden}")
-        rows = batch * seq
-        t = None
-        tp = None
-        if taps:
-            dev = x.device
-            H, Q, I = self.cfg.hidden, self.cfg.q_dim, self.cfg.intermediate
-
-            def e(*shape, dt=torch.float32):
-                return torch.empty(*shape, dtype=dt, device=dev)
-
-            f64, i8 = torch.float64, torch.int8
-            t = BlockTaps(y1=e(rows, H), q=e(rows, Q, dt=f64), attn=e(rows, Q, dt=f64),
-                          mid=e(rows, H), xq1=e(rows, H, dt=i8), amax1=e(rows),
-                          attn_norm=e(rows, Q, dt=f64), aq=e(rows, Q, dt=i8), aamax=e(rows),
-                          y2=e(rows, H), xq2=e(rows, H, dt=i8), amax2=e(rows),
-                          h=e(rows, I), hn=e(rows, I), hq=e(rows, I, dt=i8), hamax=e(rows))
-            tp = C.byref(_lib.BlockTaps(*(getattr(t, f).data_ptr() for f in BlockTaps.FIELDS)))
+        t, tp = self._taps(batch * seq, x.device) if taps else (None, None)
         check(_lib.lib().loom_amd_block_forward(self._h, C.c_void_p(x.data_ptr()), batch, seq, tp,
                                                 _stream(self.device)), "block_forward")
         return x, t
+
+    def forward_paged(self, x, cache, pages, plan, max_context: int | None = None, taps: bool = False):
+        """The block on rows x of many requests (torch float32 CUDA tensor
+        [rows, hidden], in place) over a paged 8-bit cache (paged.PagedCache)
+        instead of the block's ring: pages is the requests' table
+        (PageTable.pages) and plan the step's rows (paged.StepPlan).  Row t
+        stands at plan.positions[t] of its request; its K and V are appended to
+        the cache, and it attends to its request's tokens so far.  max_context
+        as for paged.attention.  Returns (x, BlockTaps or None)."""
+        torch = _torch()
+        if x.dtype != torch.float32 or not x.is_cuda or not x.is_contiguous():
+            raise ValueError("x must be a contiguous float32 device tensor")
+        if x.dim() != 2 or x.shape[1] != self.cfg.hidden:
+            raise ValueError(f"x must be [rows, {self.cfg.hidden}]")
+        if x.device.index != self.device or cache.device != self.device:
+            raise ValueError(f"x and cache must be on the block's device {self.device}")
+        if pages.dim() != 2 or 0 in pages.shape:
+            raise ValueError("pages must be [requests, max_pages]")
+        rows, (requests, max_pages) = x.shape[0], pages.shape
+        want = ((pages, pages.shape, "pages"), (plan.row_start, (requests + 1,), "row_start"),
+                (plan.positions, (rows,), "positions"), (plan.slots, (rows,), "slots"))
+        for a, shape, name in want:
+            if a.dtype != torch.int32 or a.device != x.device or not a.is_contiguous() or a.shape != shape:
+                raise ValueError(f"{name} must be a contiguous int32 tensor {tuple(shape)} on the block's device")
+        if max_context is None:
+            max_context = max_pages * cache.page_size
+        t, tp = self._taps(rows, x.device) if taps else (None, None)
+        check(_lib.lib().loom_amd_block_forward_paged(
+            self._h, x.data_ptr(), rows, cache._p, pages.data_ptr(), requests, max_pages, plan.row_start.data_ptr(),
+            plan.positions.data_ptr(), plan.slots.data_ptr(), max_context, tp, _stream(self.device)),
+            "block_forward_paged")
+        return x, t
+
+    def _taps(self, rows: int, dev):
+        torch = _torch()
+        H, Q, I = self.cfg.hidden, self.cfg.q_dim, self.cfg.intermediate
+
+        def e(*shape, dt=torch.float32):
+            return torch.empty(*shape, dtype=dt, device=dev)
+
+        f64, i8 = torch.float64, torch.int8
+        t = BlockTaps(y1=e(rows, H), q=e(rows, Q, dt=f64), attn=e(rows, Q, dt=f64),
+                      mid=e(rows, H), xq1=e(rows, H, dt=i8), amax1=e(rows),
+                      attn_norm=e(rows, Q, dt=f64), aq=e(rows, Q, dt=i8), aamax=e(rows),
+                      y2=e(rows, H), xq2=e(rows, H, dt=i8), amax2=e(rows),
+                      h=e(rows, I), hn=e(rows, I), hq=e(rows, I, dt=i8), hamax=e(rows))
+        return t, C.byref(_lib.BlockTaps(*(getattr(t, f).data_ptr() for f in BlockTaps.FIELDS)))
 
     def kv_cache(self, slot: int = 0):
         """(K, V) ring of one sequence slot as torch views [max_seq_len, kv_dim]."""

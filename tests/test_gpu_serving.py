@@ -1,0 +1,206 @@
+"""The serving operators together on the GPU: a block over ragged requests with
+a paged cache, stage by stage, and a serving loop of tables, block, LM head and
+sampling."""
+import numpy as np
+import pytest
+
+from tests import paged_ref as ref
+from tests.stages import BITNET_2B, SMALL, Shape, Weights, _quant, _rel_rows, f64_inner_norm
+from tests.test_gpu_paged import attention_bound, ints
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def tf(amd_lib):
+    from loom_amd import transformer
+    return transformer
+
+
+@pytest.mark.parametrize("norm", ["strict", "fast"])
+@pytest.mark.parametrize("shape,page,act,bias,qk", [(SMALL, 16, 6, False, None), (SMALL, 32, 1, True, "per_head"),
+                                                    (Shape(128, 4, 4, 32, 256, 64), 16, 6, False, "shared"),
+                                                    (BITNET_2B, 64, 1, False, None)])
+def test_block_forward_paged_stages(orc, tf, norm, shape, page, act, bias, qk):
+    """Three steps of ragged requests: the projection equals the ring block's
+    bit for bit (each request run alone through it), the cache holds those K and
+    V rows as append stores them, attention is within its bound of the formula,
+    and the stages behind it are the block's own of that attention."""
+    from loom_amd import paged
+    w = Weights(orc, shape, seed=701, act=act, bias=bias, qk=qk)
+    blk = tf.BitNetBlock(w.cfg(tf, norm), w.gpu(tf))
+    n = 5
+    table = paged.PageTable(n, 4, 4 * n, page)
+    cache = paged.PagedCache(4 * n, page, shape.kv, shape.hd)
+    kc, vc, ks, vs = (np.zeros((4 * n, shape.kv, page, shape.hd)), np.zeros((4 * n, shape.kv, page, shape.hd)),
+                      np.zeros((4 * n, shape.kv), np.float32), np.zeros((4 * n, shape.kv), np.float32))
+    lens = np.zeros(n, np.int64)
+    g = torch.Generator().manual_seed(3)
+    xs = [torch.randn(40, shape.hidden, generator=g) for _ in range(n)]
+    # the ring block over each request's whole sequence: Q, K, V of every position
+    q_all, k_all, v_all = [], [], []
+    for x in xs:
+        _, taps = blk.forward(x.cuda(), taps=True)
+        q_all.append(taps.q.cpu().numpy())
+        ck, cv = blk.kv_cache(0)
+        k_all.append(ck[:40].cpu().numpy().reshape(40, shape.kv, shape.hd))
+        v_all.append(cv[:40].cpu().numpy().reshape(40, shape.kv, shape.hd))
+    for new, pad in (([17, 1, 0, 30, 5], 2), ([1, 1, 1, 1, 1], 0), ([3, 9, 1, 0, 16], 1)):
+        new = np.array(new)
+        rows = int(new.sum()) + pad
+        plan = table.plan(ints(lens), ints(new), rows)
+        at = [(r, lens[r] + j) for r in range(n) for j in range(new[r])]
+        x_in = torch.cat([torch.stack([xs[r][p] for r, p in at]), torch.zeros(pad, shape.hidden)])
+        x, taps = blk.forward_paged(x_in.cuda(), cache, table.pages, plan, taps=True)
+        plain, _ = blk.forward_paged(x_in.cuda(), cache, table.pages, plan, max_context=64)
+        T = taps.numpy()
+        live = len(at)
+        q = np.stack([q_all[r][p] for r, p in at])
+        assert np.array_equal(T["q"][:live], q), "Q rows"
+        slots = plan.slots.cpu().numpy()
+        k, v = (np.stack([a[r][p] for r, p in at]).astype(np.float64) for a in (k_all, v_all))
+        ref.append(kc, ks, k, slots[:live])
+        ref.append(vc, vs, v, slots[:live])
+        got = cache.codes()
+        pages = table.pages.cpu().numpy()
+        lens = lens + new
+        assert np.array_equal(plan.lens.cpu().numpy(), lens)
+        for r in range(n):
+            p = np.arange(lens[r])
+            s = pages[r, p // page] * page + p % page
+            for c, want, sc, wsc in ((got[0], kc, cache.k_scale, ks), (got[1], vc, cache.v_scale, vs)):
+                assert np.array_equal(c.cpu().numpy()[s // page, :, s % page], want[s // page, :, s % page]), "codes"
+                assert np.array_equal(sc.cpu().numpy()[s // page], wsc[s // page]), "scales"
+        start = plan.row_start.cpu().numpy()
+        want = ref.attention(q.astype(np.float32).astype(np.float64).reshape(live, shape.heads, shape.hd), kc,
+                             vc.transpose(0, 1, 3, 2), ks, vs, pages, start, plan.positions.cpu().numpy(), shape.hd ** -0.5)
+        tol = attention_bound(q, kc, vc, ks, vs, shape.hd ** -0.5, 48, torch.float64)
+        assert np.abs(T["attn"][:live].reshape(want.shape) - want).max() <= tol, "attention"
+        an = f64_inner_norm(orc, T["attn"][:live], w.an)
+        if norm == "strict":
+            assert np.array_equal(T["attn_norm"][:live], an)
+        else:
+            _rel_rows(T["attn_norm"][:live], an, 1e-13, "inner norm")
+        _quant(orc, T["attn_norm"][:live], T["aq"][:live], T["aamax"][:live], "attention int8")
+        o = orc.dense_quantized(w.o, T["aq"][:live], T["aamax"][:live], bias=w.bias[3] if w.bias else None)
+        assert np.array_equal(T["mid"][:live], (o + x_in[:live].numpy()).astype(np.float32)), "O projection"
+        dn = orc.dense_quantized(w.d, T["hq"][:live], T["hamax"][:live])
+        assert np.array_equal(x[:live].cpu().numpy(), (dn + T["mid"][:live]).astype(np.float32)), "down"
+        # the same rows again (their slots are rewritten with the same values), fewer workgroups
+        assert float((plain[:live] - x[:live]).abs().max()) <= 1e-2 * float(x[:live].abs().max())
+    blk.release()
+
+
+def test_serving_loop(orc, tf):
+    """Requests come, decode at their own lengths and go: tokens, lengths and
+    pages follow the plain restatement of tables and sampling, from the same
+    logits; a request's tokens do not depend on its neighbours."""
+    from loom_amd import paged
+    sh = SMALL
+    ws = [Weights(orc, sh, seed=801 + 20 * i) for i in range(2)]
+    blocks = [tf.BitNetBlock(w.cfg(tf, "fast"), w.gpu(tf)) for w in ws]
+    vocab, slots, page = 500, 4, 16
+    g = torch.Generator().manual_seed(9)
+    emb = torch.randn(vocab, sh.hidden, generator=g).cuda()
+    prompts = [torch.randint(0, vocab, (m,), generator=g) for m in (5, 21, 1, 33, 12, 8)]
+    steps = [9, 4, 14, 3, 6, 10]
+    u_all = torch.rand(len(prompts), 20, generator=g)
+    opts = dict(temperature=[0.7, 0.0, 1.2, 0.9, 1.0, 0.5], top_k=[20, 0, 0, 5, 0, 50], top_p=[0.9, 1, 0.8, 1, 1, 0.95],
+                min_p=[0, 0, 0, 0, 0.1, 0.02])
+
+    def serve(order, width):
+        table, tables = paged.PageTable(width, 4, 3 * width + 1, page), ref.Tables(width, 4, 3 * width + 1, page)
+        caches = [paged.PagedCache(3 * width + 1, page, sh.kv, sh.hd) for _ in blocks]
+        waiting, active = list(order), [None] * width
+        out = {r: [] for r in order}
+        lens = np.zeros(width, np.int64)
+        while waiting or any(a is not None for a in active):
+            feed = []
+            for s in range(width):
+                if active[s] is None and waiting:
+                    active[s] = waiting.pop(0)
+                    lens[s] = 0
+                    feed.append(prompts[active[s]])
+                elif active[s] is not None:
+                    feed.append(torch.tensor([out[active[s]][-1]]))
+                else:
+                    feed.append(torch.zeros(0, dtype=torch.long))
+            new = np.array([len(f) for f in feed])
+            rows = int(new.sum())
+            plan = table.plan(ints(lens), ints(new), rows)
+            want = tables.plan(lens, new, rows)
+            assert np.array_equal(plan.slots.cpu().numpy(), want["slots"])
+            x = emb[torch.cat(feed).cuda()].contiguous()
+            for b, c in zip(blocks, caches):
+                b.forward_paged(x, c, table.pages, plan)
+            lens = want["lens"]
+            live = [s for s in range(width) if active[s] is not None]
+            last = plan.row_start[1:].long()[torch.tensor(live).cuda()] - 1
+            logits = tf.lm_head(emb, x[last].contiguous()) * 0.05
+            rs = [active[s] for s in live]
+            u = torch.stack([u_all[r, len(out[r])] for r in rs]).cuda()
+            args = {k: torch.tensor([v[r] for r in rs], dtype=torch.int32 if k == "top_k" else torch.float32,
+                                    device="cuda") for k, v in opts.items()}
+            ids = tf.sample(logits, u, **args).tolist()
+            lg = logits.cpu().numpy()
+            for i, r in enumerate(rs):
+                assert ids[i] == ref.sample(lg[i], np.float32(opts["temperature"][r]), opts["top_k"][r],
+                                            np.float32(opts["top_p"][r]), np.float32(opts["min_p"][r]),
+                                            np.float32(u_all[r, len(out[r])]))
+                out[r].append(ids[i])
+            done = np.array([active[s] is not None and len(out[active[s]]) >= steps[active[s]] for s in range(width)])
+            table.release(torch.tensor(done, device="cuda"))
+            tables.release(done)
+            for s in np.nonzero(done)[0]:
+                active[s], lens[s] = None, 0
+        assert int(table.free_count[0]) == 3 * width + 1
+        return out
+
+    together = serve([0, 1, 2, 3, 4, 5], slots)
+    assert [len(together[r]) for r in range(6)] == steps
+    assert serve([0, 1, 2, 3, 4, 5], slots) == together
+    for b in blocks:
+        b.release()
+
+
+def test_block_forward_paged_in_a_graph(orc, tf):
+    from loom_amd import paged
+    w = Weights(orc, SMALL, seed=811)
+    blk = tf.BitNetBlock(w.cfg(tf, "fast"), w.gpu(tf))
+    n, page = 3, 16
+
+    def fresh():
+        t, c = paged.PageTable(n, 4, 12, page), paged.PagedCache(12, page, SMALL.kv, SMALL.hd)
+        lens = ints([0, 0, 0])
+        plan = t.plan(lens, ints([5, 17, 1]), 23)
+        x = torch.randn(23, SMALL.hidden, generator=torch.Generator().manual_seed(1)).cuda()
+        blk.forward_paged(x, c, t.pages, plan)
+        return t, c, plan.lens.clone()
+
+    data = torch.randn(20, n, SMALL.hidden, generator=torch.Generator().manual_seed(2)).cuda()
+
+    def step(t, c, lens, x):
+        plan = t.plan(lens, torch.ones_like(lens), n)
+        blk.forward_paged(x, c, t.pages, plan)
+        lens.copy_(plan.lens)
+
+    t, c, lens = fresh()
+    eager = []
+    for i in range(20):
+        x = data[i].clone()
+        step(t, c, lens, x)
+        eager.append(x)
+    t, c, lens = fresh()
+    x = data[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(t, c, lens, x)
+    for i in range(20):
+        x.copy_(data[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x, eager[i]), f"replay {i}"
+    blk.release()
