@@ -439,8 +439,8 @@ int loom_amd_page_table_plan(const loom_amd_page_table* table, const int32_t* le
 int loom_amd_page_table_release(const loom_amd_page_table* table, const uint8_t* done, void* stream);
 
 /* Keys and values as int8 codes with an fp32 scale for each page, head and
- * side: value = code * scale.  Device buffers of the caller, codes 16-byte
- * aligned; head_dim 32, 64, 128 or 256. */
+ * side: value = code * scale (scales are not negative).  Device buffers of the
+ * caller, codes 16-byte aligned; head_dim 32, 64, 128 or 256. */
 typedef struct loom_amd_kv_pages {
     int8_t* k;      /* num_pages x kv_heads x page_size/16 x head_dim/16 x 16 tokens x 16 */
     int8_t* v;      /* num_pages x kv_heads x page_size/16 x head_dim x 16 tokens */
@@ -497,10 +497,11 @@ int loom_amd_paged_attention(const loom_amd_kv_pages* cache, const int32_t* page
  * attention is fp64 over fp32 rows).  pages, row_start, positions and slots as
  * a plan gives them.  The cache has the block's kv_heads and head_dim.  Rows
  * without a place have no attention; they are written like the others, and mean
- * nothing.  Independent of the block's own positions and ring.  May grow the
- * block's workspace (synchronizing the device) when rows, requests or
- * max_context exceed earlier calls: make the largest call once before a
- * capture.  Calls on one block must not overlap. */
+ * nothing.  Independent of the block's own positions and ring.  May allocate a
+ * larger workspace (waiting for the device) when rows, requests or max_context
+ * exceed earlier calls: make the largest call once before a capture; the
+ * smaller one is kept until the block is released, so calls that were captured
+ * before stay good.  Calls on one block must not overlap. */
 int loom_amd_block_forward_paged(loom_amd_block* b, float* x, int rows, const loom_amd_kv_pages* cache,
                                  const int32_t* pages, int requests, int max_pages, const int32_t* row_start,
                                  const int32_t* positions, const int32_t* slots, int max_context,

@@ -516,6 +516,7 @@ struct loom_amd_block {
     Workspace paged_ws;
     void* paged_extra = nullptr;
     size_t paged_extra_bytes = 0;
+    std::vector<void*> outgrown;  // buffers that captured graphs may still name
     int* pos = nullptr;  // device
     int shadow = 0;      // host copy of the KV position
     int warm_batch = 0;  // sequences the warm cache holds (batch of the calls that filled it)
@@ -594,6 +595,7 @@ void loom_amd_block_release(loom_amd_block* b) {
     free_workspace(&b->ws);
     free_workspace(&b->paged_ws);
     if (b->paged_extra) (void)hipFree(b->paged_extra);
+    for (void* p : b->outgrown) (void)hipFree(p);
     free_block(&b->dev);
     if (b->pos) (void)hipFree(b->pos);
     delete b;
@@ -659,25 +661,27 @@ int loom_amd_block_forward_paged(loom_amd_block* b, float* x, int rows, const lo
     hipStream_t s = (hipStream_t)stream;
     const size_t kv = ((size_t)rows * B.kv_dim * 4 + 255) & ~(size_t)255;
     const size_t extra = 2 * kv + paged_attn_workspace(rows, B.heads, B.kv_heads, B.hd, requests, max_context);
-    if (b->paged_ws.rows < rows || b->paged_extra_bytes < extra) {
-        hipError_t e = hipDeviceSynchronize();  // queued calls may still use the old workspace
-        if (e != hipSuccess) return fail_hip("block workspace", e);
-        if (b->paged_ws.rows < rows) {
-            free_workspace(&b->paged_ws);
-            if (alloc_workspace(B, rows, &b->paged_ws, true)) return -1;
-        }
-        if (b->paged_extra_bytes < extra) {
-            if (b->paged_extra) (void)hipFree(b->paged_extra);
-            b->paged_extra = nullptr;
-            b->paged_extra_bytes = 0;
-            e = hipMalloc(&b->paged_extra, extra);
-            if (e != hipSuccess) return fail_hip("block workspace", e);
-            b->paged_extra_bytes = extra;
-        }
+    if (b->paged_ws.rows < rows) {
+        // the old buffers stay: a captured call may be replayed with them
+        Workspace w;
+        if (alloc_workspace(B, rows, &w, true)) return -1;
         // a row of no request has no attention: it goes on with zeros, not with what was here
-        e = hipMemset(b->paged_ws.attn, 0, (size_t)b->paged_ws.rows * B.q_dim * 8);
+        hipError_t e = hipMemset(w.attn, 0, (size_t)rows * B.q_dim * 8);
         if (e == hipSuccess) e = hipDeviceSynchronize();
+        if (e != hipSuccess) {
+            free_workspace(&w);
+            return fail_hip("block workspace", e);
+        }
+        if (b->paged_ws.base) b->outgrown.push_back(b->paged_ws.base);
+        b->paged_ws = w;
+    }
+    if (b->paged_extra_bytes < extra) {
+        void* p = nullptr;
+        hipError_t e = hipMalloc(&p, extra);
         if (e != hipSuccess) return fail_hip("block workspace", e);
+        if (b->paged_extra) b->outgrown.push_back(b->paged_extra);
+        b->paged_extra = p;
+        b->paged_extra_bytes = extra;
     }
     pr.attn.table = pages;
     pr.attn.max_pages = max_pages;

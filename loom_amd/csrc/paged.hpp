@@ -6,10 +6,10 @@
 //   k codes: [pages][kv_heads][page / 16][head_dim / 16][16 tokens][16 dimensions]
 //   v codes: [pages][kv_heads][page / 16][head_dim][16 tokens]
 // (blocks of 16 tokens in the order in which the matrix operands of attention
-// take them: the 16 bytes of neighbouring lanes lie side by side.  Keys token by
-// token put each lane's 16 bytes into a line of its own, 64 cache accesses a
-// load instead of 16, and bound the kernel by the L1: four prompts of 2048
-// tokens 310 us)
+// take them: the 16 bytes of neighbouring lanes lie side by side.  With keys
+// token by token each lane's 16 bytes are in a line of their own, 50 cache
+// accesses a load instead of 16: four prompts of 2048 tokens took 310 us, and
+// 284 us with the blocks)
 //   scales:  [pages][kv_heads]
 // A slot is page * page_size + offset; -1 (and anything outside the cache) is
 // no slot.

@@ -812,8 +812,10 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnParams a) {
     }
 }
 
-// Parts of a context: enough workgroups to fill the chip several times over.
-constexpr int kWantGroups = 1024;
+// Parts of a context: enough workgroups to fill the chip (two of four waves a
+// CU) and even out ragged lengths; 512 and 1024 were a few per cent slower on
+// decode rows, 2048 14 % (each part has its own start and join).
+constexpr int kWantGroups = 768;
 constexpr int kMinSteps = 4;  // 256 tokens: a step for each wave of a decode workgroup
 
 static int splits_for(int rows, int heads, int kv_heads, int requests, int max_context) {

@@ -70,7 +70,7 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PageTables t, c
     __shared__ int base_s[FILL ? kFoldRequests : 1];
     __shared__ int taken_s;
     const int tid = threadIdx.x;
-    const long long free0 = *t.free_count;
+    const long long free0 = min(max(*t.free_count, 0), t.pages);  // (a table that was never reset stays in bounds)
     const long long room = (long long)t.max_pages * t.page;
     long long rows_before = 0, pages_before = 0;
     if (tid == 0) {
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PageTables t, c
         if (in) {
             base = lens[r] > 0 ? lens[r] : 0;
             n = new_tokens[r] > 0 ? new_tokens[r] : 0;
-            held = t.held[r];
+            held = min(max(t.held[r], 0), t.max_pages);
         }
         long long total;
         const long long row_end = block_scan(n, sum_rows, &total) + rows_before;
@@ -207,7 +207,7 @@ hipError_t launch_page_plan(const PageTables& t, const int32_t* lens, const int3
 __global__ __launch_bounds__(kPlanThreads) void page_release_kernel(PageTables t, const uint8_t* __restrict__ done) {
     __shared__ long long sum[kPlanWaves];
     const int tid = threadIdx.x;
-    const int free0 = *t.free_count;
+    const int free0 = min(max(*t.free_count, 0), t.pages);
     long long before = 0;
     for (int r0 = 0; r0 < t.requests; r0 += kPlanThreads) {
         const int r = r0 + tid;
@@ -259,25 +259,40 @@ __device__ __forceinline__ float finite_abs(float x) {
     return a <= kMaxFinite ? a : 0.0f;  // NaN and infinities have no part in the scale
 }
 
-// round-half-away(x / s) exactly: the estimate is at most one off, and the
-// sign of |x| - (c +- 1/2) s, one fused operation, is exact (s >= 2^-107).
-// NaN gives 0, an infinity the largest code.
-__device__ __forceinline__ int code_of(float x, float s, float inv) {
-    if (s == 0.0f) return 0;
-    const float a = fabsf(x);
-    if (!(a <= kMaxFinite)) return a != a ? 0 : (x > 0 ? 127 : -127);
-    float c = floorf(a * inv + 0.5f);
-    if (__builtin_fmaf(-(c - 0.5f), s, a) < 0.0f) c -= 1.0f;
-    else if (__builtin_fmaf(-(c + 0.5f), s, a) >= 0.0f) c += 1.0f;
-    const int i = (int)fminf(c, 127.0f);
-    return x < 0 ? -i : i;
+// round-half-away(x / s) of four finite values with |x / s| <= 127 (and a
+// rounding), exactly: the estimate is at most one off, and the sign of
+// |x| - (c +- 1/2) s, one fused operation, is exact (s >= 2^-107).  s is
+// infinite and inv 0 for a block of zeros.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float s, float inv) {
+    const float x[4] = {a, b, c, d};
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float q = x[j] * inv, m = fabsf(x[j]);
+        float h = truncf(fabsf(q) + 0.5f);
+        const float below = __builtin_fmaf(0.5f - h, s, m), above = __builtin_fmaf(-0.5f - h, s, m);
+        h += below < 0.0f ? -1.0f : (above >= 0.0f ? 1.0f : 0.0f);
+        w = __builtin_amdgcn_cvt_pk_u8_f32(copysignf(h, x[j]) + 128.0f, j, w);
+    }
+    return w ^ 0x80808080u;
 }
 
-// A code of scale `from` at the larger scale `to` (fp64: the product is exact).
-__device__ __forceinline__ int recode(int c, float from, float to) {
-    const double q = (double)c * (double)from / (double)to;
-    const int i = (int)floor(fabs(q) + 0.5);
-    return q < 0 ? -i : i;
+// Four codes of scale `from` at the larger scale `to`: round-half-away(c from /
+// to), exactly.  c from and (h +- 1/2) to are exact in fp64, so the estimate
+// (inv = 1 / to) needs no more than a comparison on either side.
+__device__ __forceinline__ uint32_t recode4(uint32_t w, double from, double to, double inv) {
+    uint32_t z = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const int c = (int8_t)(w >> (8 * b));
+        const double p = (double)abs(c) * from;
+        double h = floor(p * inv + 0.5);
+        if (p < (h - 0.5) * to) h -= 1.0;
+        else if (p >= (h + 0.5) * to) h += 1.0;
+        const int i = (int)h;
+        z |= (uint32_t)(uint8_t)(c < 0 ? -i : i) << (8 * b);
+    }
+    return z;
 }
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -306,22 +321,148 @@ __device__ __forceinline__ void load4(const T* p, bool vec, float* x) {
 
 constexpr int kWindow = 16;  // rows whose runs one workgroup looks for
 
+// One side of one head of a run of n tokens from offset `off` of a page: its
+// scale (at *scale_at), then its codes.  src is the run's first row.
+//
+// Keys: unit u is dimensions 4 (u % D4) .. of token u / D4, one word of codes.
+// Values: unit u is the same of four tokens, quad by quad, four words.  2048
+// values of a run stay in registers between the search for the largest and the
+// rounding; longer runs are read again.
+template <typename T, int HD, bool V>
+__device__ __forceinline__ void append_run(const T* src, long stride, int off, int n, int8_t* codes, float* scale_at,
+                                           bool vec, int lane) {
+    constexpr int D4 = HD / 4;
+    constexpr int PER = V ? 2 : 8;  // units of a lane in registers
+    const float had = off == 0 ? 0.0f : *scale_at;
+    const int q0 = off >> 2;
+    const int units = V ? (((off + n + 3) >> 2) - q0) * D4 : n * D4;
+    float x[8][4];
+    auto fetch = [&](int u0) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int u = u0 + lane + 64 * i;
+            const int t = V ? 4 * (q0 + u / D4) - off : u / D4;
+            const T* p = src + (long)t * stride + 4 * (u % D4);
+#pragma unroll
+            for (int j = 0; j < 8 / PER; ++j) {
+                float* y = x[V ? 4 * i + j : i];
+                if (u < units && (!V || (t + j >= 0 && t + j < n))) load4<T>(p + j * stride, vec, y);
+                else y[0] = y[1] = y[2] = y[3] = 0.0f;
+            }
+        }
+    };
+    float big = 0.0f;
+    float zero = 0.0f;  // becomes NaN with a value that is not finite
+#pragma unroll 1
+    for (int u0 = 0; u0 < units; u0 += 64 * PER) {
+        fetch(u0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                big = fmaxf(big, fabsf(x[i][j]));
+                zero = __builtin_fmaf(x[i][j], 0.0f, zero);
+            }
+        }
+    }
+    const bool odd = __any(zero != 0.0f);  // (NaN)
+    if (odd) {
+        big = 0.0f;
+#pragma unroll 1
+        for (int u0 = 0; u0 < units; u0 += 64 * PER) {
+            fetch(u0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) big = fmaxf(big, finite_abs(x[i][j]));
+            }
+        }
+    }
+    big = wave_max(big);
+    const float own = big < kTinyAmax ? 0.0f : big / 127.0f;
+    const float to = fmaxf(had, own);
+    const float inv = to > 0.0f ? 1.0f / to : 0.0f, div = to > 0.0f ? to : __builtin_inff();
+    const bool grows = off > 0 && to > had;
+    const double wide_inv = grows ? 1.0 / (double)to : 0.0;
+    if (grows) {
+        // earlier tokens (values: whole words; one shared with the run is done below)
+        const int words = V ? q0 * HD : off * D4;
+        for (int i0 = lane; i0 < words; i0 += 64 * 4) {
+            uint32_t* at[4];
+            uint32_t y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = i0 + 64 * k;
+                at[k] = (uint32_t*)(codes + (V ? v_offset(4 * (i / HD), i % HD, HD) : k_offset(i / D4, 4 * (i % D4), HD)));
+                y[k] = i < words ? *at[k] : 0u;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (i0 + 64 * k < words) *at[k] = recode4(y[k], had, to, wide_inv);
+            }
+        }
+    }
+#pragma unroll 1
+    for (int u0 = 0; u0 < units; u0 += 64 * PER) {
+        if (units > 64 * PER) fetch(u0);
+        if (odd) {
+            // NaN is stored as 0, an infinity as the largest code
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float y = x[i][j];
+                    x[i][j] = y != y ? 0.0f : copysignf(fminf(fabsf(y), fminf(127.0f * to, kMaxFinite)), y);
+                }
+            }
+        }
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            // values: word i is dimension i % 4 of unit i / 4, its bytes the tokens
+            const int r = V ? i & 4 : i, j = i & 3;
+            w[i] = V ? codes4(x[r][j], x[r + (V ? 1 : 0)][j], x[r + (V ? 2 : 0)][j], x[r + (V ? 3 : 0)][j], div, inv)
+                     : codes4(x[r][0], x[r][1], x[r][2], x[r][3], div, inv);
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int u = u0 + lane + 64 * i;
+            if (u >= units) continue;
+            if (!V) {
+                *(uint32_t*)(codes + k_offset(off + u / D4, 4 * (u % D4), HD)) = w[i];
+                continue;
+            }
+            const int q = q0 + u / D4;
+            const int t0 = 4 * q - off;  // its first token in the run
+            uint32_t mask = 0xffffffffu;
+            if (t0 < 0) mask <<= -8 * t0;
+            if (t0 + 4 > n) mask &= 0xffffffffu >> (8 * (t0 + 4 - n));
+            uint32_t* at = (uint32_t*)(codes + v_offset(4 * q, 4 * (u % D4), HD));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t z = w[(4 * i + j) & 7];
+                if (mask != 0xffffffffu) {
+                    uint32_t old = at[4 * j];
+                    if (grows && t0 < 0) old = recode4(old, had, to, wide_inv);
+                    z = (z & mask) | (old & ~mask);
+                }
+                at[4 * j] = z;
+            }
+        }
+    }
+    if (lane == 0) *scale_at = to;
+}
+
 // Jobs are (run, head, side), a wave each.  A run is the consecutive rows
 // whose slots follow one another within one page, and belongs to the window
 // of its first row.  The page's scale is the larger of what it had (unless the
 // run starts the page: then nothing of it counts any more) and the run's
 // largest magnitude / 127.  When it grows, the codes of the earlier tokens are
 // rounded again at the new scale.
-//
-// Bound by memory (one read of the rows, one write of the codes): a lane takes
-// four dimensions of a token (keys), or of four tokens (values, whose codes
-// lie token by token), in one load each, and keeps up to 2048 values of a run
-// in registers between the search for the largest and the rounding.
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void kv_append_kernel(KvPages c, const T* __restrict__ k, const T* __restrict__ v,
+__global__ __launch_bounds__(256, 3) void kv_append_kernel(KvPages c, const T* __restrict__ k, const T* __restrict__ v,
                                                         int rows, long k_stride, long v_stride, bool vec,
                                                         const int32_t* __restrict__ slots) {
-    constexpr int D4 = HD / 4;
     const int lane = threadIdx.x & 63;
     const int row0 = blockIdx.x * kWindow;
     // rows of the window that start a run
@@ -351,111 +492,14 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvPages c, const T* __re
         }
         for (; job < sides; job += waves) {
             const int head = job >> 1;
-            const bool is_v = job & 1;
-            const long stride = is_v ? v_stride : k_stride;
-            const T* src = (is_v ? v : k) + (long)row * stride + head * HD;
-            float* scale_at = (is_v ? c.v_scale : c.k_scale) + (long)page * c.kv_heads + head;
-            int8_t* codes = (is_v ? c.v : c.k) + ((long)page * c.kv_heads + head) * (long)(c.page * HD);
-            const float had = off == 0 ? 0.0f : *scale_at;
-            float x[8][4];
-            float big = 0.0f;
-            // keys: unit u is dimensions 4 (u % D4) .. of token u / D4
-            // values: unit u is four tokens of the same, quad by quad
-            const int q0 = off >> 2, quads = ((off + n + 3) >> 2) - q0;
-            const int units = is_v ? quads * D4 : n * D4;
-            const int per = is_v ? 2 : 8;  // units in registers
-            auto fetch = [&](int u0) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    int t, d;
-                    bool in;
-                    if (is_v) {
-                        const int u = u0 + lane + 64 * (i >> 2);
-                        d = 4 * (u % D4);
-                        t = 4 * (q0 + u / D4) + (i & 3) - off;
-                        in = u < units && t >= 0 && t < n;
-                    } else {
-                        const int u = u0 + lane + 64 * i;
-                        d = 4 * (u % D4);
-                        t = u / D4;
-                        in = u < units;
-                    }
-                    if (in) load4<T>(src + (long)t * stride + d, vec, x[i]);
-                    else x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
-                }
-            };
-            for (int u0 = 0; u0 < units; u0 += 64 * per) {
-                fetch(u0);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) big = fmaxf(big, finite_abs(x[i][j]));
-                }
+            const long at = (long)page * c.kv_heads + head, block = at * (c.page * HD);
+            if (job & 1) {
+                append_run<T, HD, true>(v + (long)row * v_stride + head * HD, v_stride, off, n, c.v + block, c.v_scale + at,
+                                        vec, lane);
+            } else {
+                append_run<T, HD, false>(k + (long)row * k_stride + head * HD, k_stride, off, n, c.k + block,
+                                         c.k_scale + at, vec, lane);
             }
-            big = wave_max(big);
-            const float own = big < kTinyAmax ? 0.0f : big / 127.0f;
-            const float to = fmaxf(had, own);
-            const float inv = to > 0.0f ? 1.0f / to : 0.0f;
-            const bool grows = off > 0 && to > had;
-            if (grows) {
-                if (is_v) {  // whole words of earlier tokens (a word shared with the run is done below)
-                    for (int i = lane; i < q0 * HD; i += 64) {
-                        uint32_t* at = (uint32_t*)(codes + v_offset(4 * (i / HD), i % HD, HD));
-                        uint32_t w = *at, z = 0;
-#pragma unroll
-                        for (int b = 0; b < 4; ++b) z |= (uint32_t)(uint8_t)recode((int8_t)(w >> (8 * b)), had, to) << (8 * b);
-                        *at = z;
-                    }
-                } else {
-                    for (int i = lane; i < off * D4; i += 64) {
-                        uint32_t* at = (uint32_t*)(codes + k_offset(i / D4, 4 * (i % D4), HD));
-                        uint32_t w = *at, z = 0;
-#pragma unroll
-                        for (int b = 0; b < 4; ++b) z |= (uint32_t)(uint8_t)recode((int8_t)(w >> (8 * b)), had, to) << (8 * b);
-                        *at = z;
-                    }
-                }
-            }
-            for (int u0 = 0; u0 < units; u0 += 64 * per) {
-                if (units > 64 * per) fetch(u0);
-                if (is_v) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int u = u0 + lane + 64 * i;
-                        if (u >= units) continue;
-                        const int q = q0 + u / D4;
-                        const int t0 = 4 * q - off;
-                        const bool whole = t0 >= 0 && t0 + 4 <= n;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t* at = (uint32_t*)(codes + v_offset(4 * q, 4 * (u % D4) + j, HD));
-                            uint32_t w = whole ? 0u : *at, z = 0;
-#pragma unroll
-                            for (int b = 0; b < 4; ++b) {
-                                int code = (int8_t)(w >> (8 * b));
-                                if (t0 + b < 0) {
-                                    if (grows) code = recode(code, had, to);
-                                } else if (t0 + b < n) {
-                                    code = code_of(x[4 * i + b][j], to, inv);
-                                }
-                                z |= (uint32_t)(uint8_t)code << (8 * b);
-                            }
-                            *at = z;
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int u = u0 + lane + 64 * i;
-                        if (u >= units) continue;
-                        uint32_t z = 0;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) z |= (uint32_t)(uint8_t)code_of(x[i][j], to, inv) << (8 * j);
-                        *(uint32_t*)(codes + k_offset(off + u / D4, 4 * (u % D4), HD)) = z;
-                    }
-                }
-            }
-            if (lane == 0) *scale_at = to;
         }
     }
 }

@@ -35,7 +35,7 @@ import functools
 
 from . import _lib
 from ._lib import check
-from .bitnet import _stream, _torch
+from .bitnet import _torch
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (32, 64, 128, 256)
@@ -52,34 +52,36 @@ def _index(device) -> int:
     return torch.cuda.current_device() if d.index is None else d.index
 
 
+# (Host time counts here: a decode step's calls take the GPU 5 to 15 us each.
+# Tensor.get_device and the raw device and stream getters are a fraction of the
+# objects that Tensor.device and torch.cuda.current_device go through.)
+
 def _device_of(t, what: str) -> int:
-    if not t.is_cuda:
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError(f"{what} must be a device tensor")
-    return t.device.index
+    return dev
 
 
 def _want(t, dtype, shape, dev: int, what: str):
     """A contiguous tensor of this dtype, shape (None: any) and device."""
-    if t.dtype != dtype or not t.is_cuda or t.device.index != dev or not t.is_contiguous():
+    if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {str(dtype).split('.')[-1]} tensor on device {dev}")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{what} is {tuple(t.shape)}, want {tuple(shape)}")
     return t.data_ptr()
 
 
-def on_device(dev: int):
-    """Context that makes dev current (nothing to do when it is)."""
-    torch = _torch()
-    return torch.cuda.device(dev)
-
-
 def _call(dev: int, what: str, fn, *args) -> None:
     """fn(*args, stream) on device dev's current stream."""
-    if _torch().cuda.current_device() == dev:
-        check(fn(*args, _stream(dev)), what)
+    torch = _torch()
+    if torch._C._cuda_getDevice() == dev:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with on_device(dev):
-            check(fn(*args, _stream(dev)), what)
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(rc, what)
 
 
 def _rows_type() -> dict:
@@ -167,7 +169,7 @@ class PageTable:
         if rows < 0:
             raise ValueError("rows must not be negative")
         buf = torch.empty(6 * n + 1 + 3 * rows, dtype=torch.int32, device=lens.device)
-        scratch, start, after, req, pos, slots = buf.split((4 * n, n + 1, n, rows, rows, rows))
+        scratch, start, after, req, pos, slots = buf.split_with_sizes((4 * n, n + 1, n, rows, rows, rows))
         at = buf.data_ptr()
         at1 = at + 16 * n
         at2 = at1 + 4 * n + 4
@@ -214,7 +216,8 @@ class PagedCache:
     def from_tensors(cls, k, v, k_scale, v_scale) -> "PagedCache":
         """A cache that holds these codes and scales: k int8 [num_pages,
         kv_heads, page_size, head_dim], v int8 [num_pages, kv_heads, head_dim,
-        page_size], scales float32 [num_pages, kv_heads].  They are copied."""
+        page_size], scales float32 [num_pages, kv_heads], none negative.  They
+        are copied."""
         torch = _torch()
         if k.dim() != 4:
             raise ValueError("k must be [num_pages, kv_heads, page_size, head_dim]")
@@ -285,12 +288,19 @@ class PagedCache:
         return k, v
 
 
-@functools.lru_cache(maxsize=4096)
-def _attention_workspace(rows, heads, kv_heads, head_dim, requests, max_context) -> int:
-    n = C.c_size_t()
-    check(_lib.lib().loom_amd_paged_attention_workspace(rows, heads, kv_heads, head_dim, requests, max_context,
-                                                        C.byref(n)), "paged_attention")
-    return n.value
+_workspaces: dict = {}
+
+
+def _attention_workspace(*shape) -> int:
+    """Bytes of workspace for (rows, heads, kv_heads, head_dim, requests, max_context)."""
+    need = _workspaces.get(shape)
+    if need is None:
+        n = C.c_size_t()
+        check(_lib.lib().loom_amd_paged_attention_workspace(*shape, C.byref(n)), "paged_attention")
+        if len(_workspaces) >= 4096:
+            _workspaces.clear()
+        need = _workspaces[shape] = n.value
+    return need
 
 
 def attention(q, cache: PagedCache, pages, row_start, positions, scale: float | None = None,

@@ -337,7 +337,7 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
         if t is None and name != "uniform":
             args.append(None)
             continue
-        if t.dtype != dt or t.device != logits.device or t.shape != (rows,) or not t.is_contiguous():
+        if t is None or t.dtype != dt or t.device != logits.device or t.shape != (rows,) or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous {str(dt).split('.')[-1]} tensor of {rows} values on "
                              f"the logits' device")
         args.append(t.data_ptr())
@@ -345,7 +345,7 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
     need = _sample_workspace(vocab, rows)
     ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
     call = (logits.data_ptr(), logits.stride(0), vocab, rows, *args, ids.data_ptr(), ws.data_ptr(), need)
-    if torch.cuda.current_device() == dev:
+    if torch._C._cuda_getDevice() == dev:
         check(_lib.lib().loom_amd_sample(*call, _stream(dev)), "sample")
     else:
         with torch.cuda.device(dev):

@@ -204,3 +204,84 @@ def test_block_forward_paged_in_a_graph(orc, tf):
         torch.cuda.synchronize()
         assert torch.equal(x, eager[i]), f"replay {i}"
     blk.release()
+
+
+def test_block_forward_paged_growing_and_refusals(orc, tf):
+    """A larger call after a capture leaves the captured one good; a cache of
+    another shape and tensors of other types are refused."""
+    from loom_amd import _lib, paged
+    w = Weights(orc, SMALL, seed=821)
+    blk = tf.BitNetBlock(w.cfg(tf, "fast"), w.gpu(tf))
+    t, c = paged.PageTable(2, 8, 16, 16), paged.PagedCache(16, 16, SMALL.kv, SMALL.hd)
+    lens, one = ints([0, 0]), ints([1, 1])
+    plan = t.plan(lens, one, 2)
+    x0 = torch.randn(2, SMALL.hidden, generator=torch.Generator().manual_seed(3)).cuda()
+    x = x0.clone()
+    blk.forward_paged(x, c, t.pages, plan)
+    want = x.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        blk.forward_paged(x, c, t.pages, plan)
+    big = t.plan(ints([1, 1]), ints([100, 90]), 200)
+    y = torch.randn(200, SMALL.hidden, generator=torch.Generator().manual_seed(4)).cuda()
+    blk.forward_paged(y, c, t.pages, big)
+    for _ in range(3):
+        x.copy_(x0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x, want)
+    with pytest.raises(_lib.AMDError, match="heads"):
+        blk.forward_paged(x, paged.PagedCache(16, 16, SMALL.kv + 1, SMALL.hd), t.pages, plan)
+    with pytest.raises(_lib.AMDError, match="max_context"):
+        blk.forward_paged(x, c, t.pages, plan, max_context=1000)
+    for bad in (x.half(), x[:1], x[:, :8], x.t()):
+        with pytest.raises(ValueError):
+            blk.forward_paged(bad, c, t.pages, plan)
+    with pytest.raises(ValueError, match="slots"):
+        blk.forward_paged(x, c, t.pages, paged.StepPlan(plan.row_start, plan.lens, plan.request, plan.positions,
+                                                        plan.slots.long()))
+    blk.release()
+
+
+def test_refusals_of_device_tensors(tf):
+    from loom_amd import paged
+    c = paged.PagedCache(4, 16, 2, 64)
+    q, k = torch.zeros(3, 4, 64, device="cuda"), torch.zeros(3, 2, 64, device="cuda")
+    pages, start, pos = ints([[0, 1]]), ints([0, 3]), ints([0, 1, 2])
+    good = dict(q=q, cache=c, pages=pages, row_start=start, positions=pos)
+    assert not paged.attention(**good).any()
+    for kw in (dict(q=q.half()), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(q=q.cpu()), dict(q=q[:1].expand(3, 4, 64)),
+               dict(q=torch.zeros(3, 64, 4, device="cuda").transpose(1, 2)), dict(pages=pages.long()), dict(pages=pages[0]),
+               dict(pages=pages[:, :0]), dict(row_start=start[:1]), dict(positions=pos[:2]), dict(positions=pos.cpu()),
+               dict(max_context=33), dict(max_context=-1), dict(out=torch.zeros(3, 4, 64)), dict(out=q[:2]),
+               dict(out=torch.zeros(1, 4, 64, device="cuda").expand(3, 4, 64))):
+        with pytest.raises(ValueError):
+            paged.attention(**{**good, **kw})
+    slots = ints([0, 1, 2])
+    for a in ((k, k.bfloat16(), slots), (k.half(), k.half(), slots), (k, k, slots.long()), (k[:2], k, slots),
+              (k.cpu(), k.cpu(), slots), (k[:1].expand(3, 2, 64), k, slots)):
+        with pytest.raises(ValueError):
+            c.append(*a)
+    for a in (slots.long(), slots.cpu(), slots[None]):
+        with pytest.raises(ValueError):
+            c.read(a)
+    t = paged.PageTable(2, 3, 4)
+    for a in ((ints([0]), ints([1, 1]), 2), (ints([0, 0]), ints([1, 1]).long(), 2), (ints([0, 0]), ints([1, 1]).cpu(), 2),
+              (ints([0, 0]), ints([1, 1]), -1)):
+        with pytest.raises(ValueError):
+            t.plan(*a)
+    with pytest.raises(ValueError):
+        t.release(ints([0, 1]))
+    lg, u = torch.zeros(2, 10, device="cuda"), torch.zeros(2, device="cuda")
+    for a, kw in (((lg.half(), u), {}), ((lg[0], u), {}), ((lg.t(), u), {}), ((lg, u[:1]), {}), ((lg, u.cpu()), {}),
+                  ((lg, None), {}), ((lg, u), dict(top_k=u)), ((lg, u), dict(temperature=u.double())),
+                  ((lg[:1].expand(2, 10), u), {})):
+        with pytest.raises(ValueError):
+            tf.sample(*a, **kw)
+    # no rows at all
+    none = ints([])
+    assert paged.attention(q[:0], c, pages, ints([0, 0]), none).shape == (0, 4, 64)
+    c.append(k[:0], k[:0], none)
+    assert c.read(none)[0].shape == (0, 2, 64)
+    assert tf.sample(lg[:0], u[:0]).shape == (0,)
