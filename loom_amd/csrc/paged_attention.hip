@@ -6,10 +6,11 @@
 // over t <= position(row), with k_t = kc_t ks, v_t = vc_t vs of t's page.
 //
 // The matrix cores read the keys' codes as they are stored: q is written in
-// fixed point as QD signed 8-bit digits relative to its largest magnitude, and
-// v_mfma_i32_16x16x64_i8 forms every digit's dot product exactly in 32 bits;
-// the digits' sums are joined in fp32.  Three digits (23 bits and sign) leave
-// no more error than an fp32 q has; two (15 bits) stand far below a bf16 q's.
+// fixed point as three signed 8-bit digits (23 bits and sign) of its largest
+// magnitude, and v_mfma_i32_16x16x64_i8 forms every digit's dot product exactly
+// in 32 bits; the digits' sums are joined in fp32.  That is no more error than
+// an fp32 product has.  (Two digits would do for bf16 rows without outliers;
+// they saved nothing on decode rows and 4 % on chunks.)
 // The values' codes become fp16 (exact) and meet p as one fp16 factor (bf16
 // rows) or as the sum of two (22 bits, fp32 rows).
 //
@@ -30,6 +31,7 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kStep = 64;         // tokens of one step
+constexpr int QD = 3;             // digits of q
 constexpr int kMaxSplits = 64;    // parts of one context (a wave joins them, a lane each)
 // fp16 value of a probability of 1, and how far (log2) a score may pass the
 // maximum that the sums are relative to before they are rescaled: 2^(9 + 6)
@@ -178,7 +180,7 @@ __device__ __forceinline__ int find_request(const AttnParams& a, int ct, int x, 
 }
 
 // 16 columns of one wave.
-template <int HD, int QD, int PL>
+template <int HD, int PL>
 struct Wave {
     static constexpr int NS = HD >= 64 ? HD / 64 : 1;  // 64-dimension steps of the score product
     static constexpr int ND = HD / 16;                 // 16-dimension tiles of the output
@@ -210,8 +212,8 @@ struct Wave {
         }
         big = column_max(big);
         const float nan = column_sum(bad ? __builtin_nanf("") : 0.0f);
-        // largest fixed-point value: just under the digits' own, 127 * (1 + 256 (+ 65536))
-        constexpr float kTop = QD == 3 ? 8355000.0f : 32600.0f;
+        // largest fixed-point value: just under the digits' own, 127 * (1 + 256 + 65536)
+        constexpr float kTop = 8355000.0f;
         const bool zero = big < 0x1p-100f;
         const float inv = zero ? 0.0f : (a.scale2 < 0.0f ? -kTop : kTop) / big;
         qf = (zero ? 0.0f : big / kTop) * fabsf(a.scale2);
@@ -231,11 +233,9 @@ struct Wave {
                 const uint32_t a23 = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
                 qd[0][s][w] = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100u);
                 qd[1][s][w] = (int)__builtin_amdgcn_perm(a23, a01, 0x07060302u);
-                if (QD == 3) {
-                    const uint32_t b01 = __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0602u);
-                    const uint32_t b23 = __builtin_amdgcn_perm(y[3], y[2], 0x0c0c0602u);
-                    qd[QD - 1][s][w] = (int)__builtin_amdgcn_perm(b23, b01, 0x05040100u);
-                }
+                const uint32_t b01 = __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0602u);
+                const uint32_t b23 = __builtin_amdgcn_perm(y[3], y[2], 0x0c0c0602u);
+                qd[2][s][w] = (int)__builtin_amdgcn_perm(b23, b01, 0x05040100u);
             }
         }
     }
@@ -263,8 +263,7 @@ struct Wave {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             // (a digit's sum is at most 2^22 at head_dim 256: 256 times that fits)
-            const float top = (float)(acc[QD - 1][i] * 256 + acc[QD - 2][i]);
-            x[i] = QD == 3 ? __builtin_fmaf(top, 256.0f, (float)acc[0][i]) : top;
+            x[i] = __builtin_fmaf((float)(acc[2][i] * 256 + acc[1][i]), 256.0f, (float)acc[0][i]);
         }
     }
 
@@ -419,10 +418,12 @@ __device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f 
 // cache's bytes: codes go straight to registers, each read once, the next
 // step's under way while this one's are used.  (Row r of the key operand of
 // tile t is token 16 (r >> 2) + 4 t + (r & 3): a lane's 16 scores are those of
-// the 16 tokens whose values it holds, in one page.)
-template <int HD, int QD, int PL>
+// the 16 tokens whose values it holds, in one page.)  Seven contexts of 65536
+// tokens, 5 heads of 128: 113 us, 5.2 TB/s; 64 rows of up to 4096 tokens 40 us,
+// 4.7 TB/s.
+template <int HD, int PL>
 __global__ __launch_bounds__(256) void paged_attn_rows_kernel(AttnParams a) {
-    using W = Wave<HD, QD, PL>;
+    using W = Wave<HD, PL>;
     constexpr int NS = W::NS, ND = W::ND;
     constexpr int LDO = HD + 4;
     __shared__ __align__(16) float o_s[4 * 16 * LDO];
@@ -430,8 +431,9 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(AttnParams a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.y, part = blockIdx.z;
-    int first_tile;
-    const int r = find_request(a, 16, blockIdx.x, lane, &first_tile);
+    // beside the chunk kernel a request has one tile here or none: no search
+    int first_tile = blockIdx.x;
+    const int r = a.hi_cols == 16 ? blockIdx.x : find_request(a, 16, blockIdx.x, lane, &first_tile);
     if (r < 0) return;
     int start = a.row_start[r], end = a.row_start[r + 1];
     start = start < 0 ? 0 : start;
@@ -570,21 +572,24 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(AttnParams a) {
     }
 }
 
-// Many columns of one request (chunks of prompts): eight waves of 16 columns
+// Many columns of one request (chunks of prompts): four waves of 16 columns
 // each go through the part's steps together.  Bound by vector instructions
 // (about 15 for each score, exp2 among them), so what the waves can share is
 // done once: a step's codes are staged in LDS, keys as stored, values as fp16,
 // in the order of the operands (whole-line reads without bank conflicts), and
-// few enough registers stay that four waves share a SIMD (head_dim up to 128).
+// few enough registers stay that three waves share a SIMD (head_dim up to 128;
+// eight waves of 128 columns at four a SIMD spilled: 319 us).
 // Row r of the key operand of tile t is token 16 t + r here: a lane's scores
 // are tokens 16 t + 4 g + i, and the values' tokens are written in that order.
 // Two buffers, one barrier a step.
 constexpr int kChunkWaves = 4;
 constexpr int kChunkCols = 16 * kChunkWaves;
 
-template <int HD, int QD, int PL>
+// (Four prompts of 2048 tokens, 20 heads of 128, fp32: 255 us, 335 TFLOP/s; the
+// same tiles with codes straight to registers 284.)
+template <int HD, int PL>
 __global__ __launch_bounds__(64 * kChunkWaves, HD <= 128 ? 3 : 1) void paged_attn_chunk_kernel(AttnParams a) {
-    using W = Wave<HD, QD, PL>;
+    using W = Wave<HD, PL>;
     constexpr int NS = W::NS, ND = W::ND, THREADS = 64 * kChunkWaves;
     constexpr int KU = 4 * HD;                           // 16-byte units of a step's keys, and of its values
     constexpr int PER = (2 * KU + THREADS - 1) / THREADS;  // units of a thread
@@ -846,19 +851,20 @@ size_t paged_attn_workspace(int rows, int heads, int kv_heads, int hd, int reque
     return part_layout(rows, heads, hd, splits_for(rows, heads, kv_heads, requests, max_context)).bytes;
 }
 
-template <int HD, int QD, int PL>
+template <int HD, int PL>
 static hipError_t launch_typed(AttnParams& a, hipStream_t s) {
     const long cols = (long)a.rows * a.group;
     // requests of at most 16 columns (decode rows) take the rows kernel; where
     // every request may be one, it takes all of them
     const bool few = cols <= 16l * a.requests;
     a.hi_cols = few ? 0x7fffffff : 16;
-    hipLaunchKernelGGL((paged_attn_rows_kernel<HD, QD, PL>),
-                       dim3((unsigned)(cols / 16 + a.requests), (unsigned)a.kv_heads, (unsigned)a.splits), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_attn_rows_kernel<HD, PL>),
+                       dim3((unsigned)(few ? cols / 16 + a.requests : a.requests), (unsigned)a.kv_heads, (unsigned)a.splits),
+                       dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (!few) {
-        hipLaunchKernelGGL((paged_attn_chunk_kernel<HD, QD, PL>),
+        hipLaunchKernelGGL((paged_attn_chunk_kernel<HD, PL>),
                            dim3((unsigned)(cols / kChunkCols + a.requests), (unsigned)a.kv_heads, (unsigned)a.splits),
                            dim3(64 * kChunkWaves), 0, s, a);
         e = hipGetLastError();
@@ -905,7 +911,7 @@ hipError_t launch_paged_attn(const PagedAttn& p, hipStream_t s) {
     a.part_ml = (float*)((char*)p.workspace + l.ml);
     a.active = (int32_t*)((char*)p.workspace + l.active);
 #define ATTN(HD) \
-    case HD: return p.type == ROW_BF16 ? launch_typed<HD, 2, 1>(a, s) : launch_typed<HD, 3, 2>(a, s);
+    case HD: return p.type == ROW_BF16 ? launch_typed<HD, 1>(a, s) : launch_typed<HD, 2>(a, s);
     switch (p.c.hd) {
         ATTN(32)
         ATTN(64)

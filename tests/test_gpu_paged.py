@@ -178,10 +178,10 @@ def test_append_not_finite_and_tiny(paged):
 def attention_bound(q, kc, vc, ks, vs, scale, longest, dtype):
     """How far a row may be off, from its scores' and sums' roundings.
 
-    Scores: q in fixed point is off by at most half a unit of amax / 8355000
-    (fp32 rows, 3 digits) or amax / 32600 (bf16, 2 digits); the digits' sums are
-    exact, their join and factors take 7 roundings, the difference to the
-    maximum 1 more of up to twice the score: 9 * 2^-24 |s| in all.
+    Scores: q in fixed point is off by at most half a unit of amax / 8355000;
+    the digits' sums are exact, their join and factors take 7 roundings, the
+    difference to the maximum 1 more of up to twice the score: 9 * 2^-24 |s| in
+    all.
     A probability is off by that, 2^-23 of exp2 and its fp16 form (2^-22 as a
     pair, 2^-12 as one); numerator and denominator both: twice.  The sums: 16
     terms and 4 products a step of 64 tokens, and the join, each 2^-23 at most.
@@ -189,7 +189,7 @@ def attention_bound(q, kc, vc, ks, vs, scale, longest, dtype):
     big_k = np.abs(kc).astype(np.float64).sum(-1).max(initial=0) * np.nanmax(ks)
     big_q = np.abs(q[np.isfinite(q)]).max(initial=0)
     s = big_q * scale * big_k * 0.5  # (a loose bound of |q.k|)
-    unit = 0.5 / (8355000 if dtype != torch.bfloat16 else 32600)
+    unit = 0.5 / 8355000
     d = big_q * unit * scale * big_k + 9 * 2.0 ** -24 * s + 2.0 ** -23
     d += 2.0 ** -22 if dtype != torch.bfloat16 else 2.0 ** -12
     d = 2 * d + (longest / 64 * 20 + 40) * 2.0 ** -23

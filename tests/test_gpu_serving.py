@@ -285,3 +285,67 @@ def test_refusals_of_device_tensors(tf):
     c.append(k[:0], k[:0], none)
     assert c.read(none)[0].shape == (0, 2, 64)
     assert tf.sample(lg[:0], u[:0]).shape == (0,)
+
+
+def test_calls_on_two_streams_at_once(tf):
+    """Attention and sampling with their workspaces on two streams at once give
+    what each gives alone (contexts long enough to be cut into parts)."""
+    from loom_amd import paged
+    c = paged.PagedCache(400, 16, 2, 64)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for t in (c.k, c.v):
+        t.copy_(torch.randint(-127, 128, t.shape, generator=g, device="cuda"))
+    c.k_scale.fill_(0.01)
+    c.v_scale.fill_(0.02)
+    pages = torch.randperm(400, generator=g, device="cuda").to(torch.int32).view(2, 200)
+    start, pos = ints([0, 1, 2]), ints([3100, 2400])
+    qs = torch.randn(8, 2, 8, 64, generator=g, device="cuda")
+    lg = torch.randn(8, 3, 30000, generator=g, device="cuda")
+    u = torch.rand(8, 3, generator=g, device="cuda")
+    p = torch.tensor([0.9, 0.5, 1.0], device="cuda")
+    want = [(paged.attention(qs[i], c, pages, start, pos), tf.sample(lg[i], u[i], top_p=p)) for i in range(8)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None] * 8
+    for rep in range(4):
+        for i in range(8):
+            with torch.cuda.stream(streams[i % 2]):
+                got[i] = (paged.attention(qs[i], c, pages, start, pos), tf.sample(lg[i], u[i], top_p=p))
+        torch.cuda.synchronize()
+        for i in range(8):
+            assert torch.equal(got[i][0], want[i][0]) and torch.equal(got[i][1], want[i][1]), (rep, i)
+
+
+def test_two_graphs_replayed_in_turn_and_at_once(tf):
+    from loom_amd import paged
+    c = paged.PagedCache(300, 32, 1, 128)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for t in (c.k, c.v):
+        t.copy_(torch.randint(-127, 128, t.shape, generator=g, device="cuda"))
+    c.k_scale.fill_(0.01)
+    c.v_scale.fill_(0.02)
+    pages = torch.randperm(300, generator=g, device="cuda").to(torch.int32).view(2, 150)
+    calls = []
+    for i, (start, pos) in enumerate(((ints([0, 1, 2]), ints([4000, 3500])), (ints([0, 40, 41]), torch.cat(
+            [torch.arange(1000, 1040, device="cuda"), torch.tensor([4500], device="cuda")]).to(torch.int32)))):
+        q = torch.randn(pos.shape[0], 4, 128, generator=g, device="cuda")
+        want = paged.attention(q, c, pages, start, pos).clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = paged.attention(q, c, pages, start, pos)
+        calls.append((graph, out, want, (q, start, pos)))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for rep in range(5):
+        for graph, out, want, _ in calls:
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+        for (graph, out, _, _), s in zip(calls, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, out, want, _ in calls:
+            assert torch.equal(out, want), rep
